@@ -73,11 +73,17 @@ class GhMlstm(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("heads", "dim", "vdim")] + [("gate_cap", C.c_float), ("eps", C.c_float)]
 
 
+class GhPages(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("page_stride", C.c_uint64), ("n_pages", C.c_uint32), ("page_tokens", C.c_uint32), ("table", C.c_void_p),
+                ("table_stride", C.c_uint32)]
+
+
 _lib: Optional[C.CDLL] = None
 
 # name -> (restype, argtypes); every symbol declared in include/glint_hip.h
 _u64, _u32, _vp, _i, _f = C.c_uint64, C.c_uint32, C.c_void_p, C.c_int, C.c_float
 _shp = C.POINTER(GhShape)
+_pgs = C.POINTER(GhPages)
 _step, _win, _mls = C.POINTER(GhStreamStep), C.POINTER(GhWindowAttn), C.POINTER(GhMlstm)
 SIGNATURES = {
     "gh_init": (_i, [_i]),
@@ -172,6 +178,15 @@ SIGNATURES = {
     "gh_attn_set_prefill_tiles": (_i, [_i]),
     "gh_attn_prefill_workspace": (_u64, [_u64, _u32, _shp]),
     "gh_attn_prefill": (_i, [_vp, _vp, _vp, _vp, _u64, _u32, _u32, _shp, _i, _vp, _u64, _i, _vp]),
+    "gh_page_rows": (_i, [_pgs, _vp, _vp, _u64, _u64, _u32, _vp, _vp, _i, _vp]),
+    "gh_attn_decode_paged_workspace": (_u64, [_u64, _u32, _shp, _i]),
+    "gh_attn_decode_paged": (_i, [_vp, _pgs, _vp, _vp, _u64, _u32, _shp, _i, _vp, _u64, _vp]),
+    "gh_attn_packed_workspace": (_u64, [_u64, _u64, _u32, _shp, _i]),
+    "gh_attn_packed": (_i, [_vp, _pgs, _vp, _vp, _vp, _u64, _u64, _u32, _shp, _i, _vp, _u64, _vp]),
+    "gh_copy_pages": (_i, [_vp, _u64, _u64, _u32, _u64, _u64, _vp, _u64, _vp]),
+    "gh_copy_pages_host": (_i, [_vp, _u64, _u64, _u32, _u64, _u64, _vp, _u64, _vp]),
+    "gh_token_logprobs_workspace": (_u64, [_u64, _u64, _u32]),
+    "gh_token_logprobs": (_i, [_vp, _vp, _vp, _vp, _vp, _u64, _vp, _u64, _u64, _u32, _i, _vp, _u64, _vp]),
     "gh_embed_step": (_i, [_vp, _vp, _vp, _u64, _u64, _u64, _u64, _u32, _vp, _vp, _u64, _u64, _u64, _vp, _u64, _step, _i, _vp]),
     "gh_matmul_scaled_argmax": (_i, [_vp, _vp, _vp, _vp, _u64, _u64, _u64, _f, _i, _vp]),
     "gh_embed_positions": (_i, [_vp, _vp, _vp, _u64, _u32, _vp, _vp, _u64, _u64, _u64, _vp, _u64, _i, _vp]),

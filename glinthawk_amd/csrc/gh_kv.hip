@@ -169,7 +169,7 @@ int gh_kv_append( void* const* token_rows_dev, const void* state_kv, uint64_t ba
     return GH_OK;
   }
   GH_REQUIRE( token_rows_dev && state_kv, "gh_kv_append: NULL pointer" );
-  GH_REQUIRE( dt == GH_F16 || dt == GH_F32, "gh_kv_append: unsupported dtype %d", (int)dt );
+  GH_REQUIRE( dt == GH_F16 || dt == GH_F32 || dt == GH_BF16, "gh_kv_append: unsupported dtype %d", (int)dt );
   GH_REQUIRE( kv_dim > 0 && batch <= 65535, "gh_kv_append: bad shape" );
   const uint32_t row_bytes = 2u * kv_dim * (uint32_t)dtype_size( dt );
   const unsigned bx = ( row_bytes / 16 + 255 ) / 256;
@@ -226,6 +226,9 @@ int gh_rope( uint64_t batch, const uint32_t* pos_dev, const void* freq_real, con
   } else if ( dt == GH_F32 ) {
     rope_kernel<float><<<grid, 256, 0, as_stream( stream )>>>( pos_dev, static_cast<const float*>( freq_real ), static_cast<const float*>( freq_imag ),
                                                              static_cast<float*>( q ), token_rows_dev, n_kv_heads, gqa_size, head_size );
+  } else if ( dt == GH_BF16 ) {
+    rope_kernel<__bf16><<<grid, 256, 0, as_stream( stream )>>>( pos_dev, static_cast<const __bf16*>( freq_real ), static_cast<const __bf16*>( freq_imag ),
+                                                              static_cast<__bf16*>( q ), token_rows_dev, n_kv_heads, gqa_size, head_size );
   } else {
     return fail( GH_ERR_INVALID, "gh_rope: unsupported dtype %d", (int)dt );
   }

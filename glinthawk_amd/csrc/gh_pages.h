@@ -1,0 +1,188 @@
+// What the kernels over a paged cache share: the address of a token's row, the sequence and tokens of a work-group's block, the walk over
+// the keys of one query row, and the checks of a description of pages.
+#pragma once
+
+#include "gh_common.h"
+
+namespace gh {
+
+struct Pages
+{
+  const char* pool;
+  uint64_t stride; // bytes from page to page
+  uint32_t last;   // number of the last page
+  uint32_t shift;  // page_tokens = 1 << shift
+  const uint32_t* table;
+  uint32_t table_stride;
+  uint32_t row_bytes;
+
+  // a page number that the pool does not have reads as its last page
+  __host__ __device__ __forceinline__ const char* page( uint32_t seq, uint32_t index ) const
+  {
+    const uint32_t number = table[(uint64_t)seq * table_stride + index];
+    return pool + ( number < last ? number : last ) * stride;
+  }
+  __host__ __device__ __forceinline__ const char* row( uint32_t seq, uint32_t key ) const
+  {
+    return page( seq, key >> shift ) + (uint64_t)( key & ( ( 1u << shift ) - 1 ) ) * row_bytes;
+  }
+  // keys that the table reaches (below 2^31, see check_pages)
+  __host__ __device__ __forceinline__ uint32_t reach() const { return table_stride << shift; }
+};
+
+// Checks a caller's description and gives the kernels' form of it.
+inline int check_pages( const char* op, const gh_pages* p, uint64_t kv_dim, gh_dtype dt, Pages* out )
+{
+  GH_REQUIRE( dt == GH_F16 || dt == GH_F32 || dt == GH_BF16, "%s: unsupported dtype %d", op, (int)dt );
+  GH_REQUIRE( p != nullptr && p->pool && p->table, "%s: NULL pages", op );
+  const uint64_t size = dtype_size( dt );
+  GH_REQUIRE( kv_dim > 0 && kv_dim <= 1u << 24, "%s: bad kv_dim", op );
+  GH_REQUIRE( p->n_pages > 0 && p->table_stride > 0, "%s: no pages", op );
+  GH_REQUIRE( p->page_tokens > 0 && ( p->page_tokens & ( p->page_tokens - 1 ) ) == 0, "%s: a page of %u tokens is no power of two", op, p->page_tokens );
+  const uint64_t page_bytes = 2 * kv_dim * size * p->page_tokens;
+  GH_REQUIRE( page_bytes < 1ull << 31, "%s: a page of %llu bytes (2 GiB and more)", op, (unsigned long long)page_bytes );
+  GH_REQUIRE( p->page_stride >= page_bytes && p->page_stride % size == 0 && p->page_stride < 1ull << 40, "%s: pages of %llu bytes lie %llu apart", op,
+              (unsigned long long)page_bytes, (unsigned long long)p->page_stride );
+  GH_REQUIRE( reinterpret_cast<uintptr_t>( p->pool ) % size == 0 && reinterpret_cast<uintptr_t>( p->table ) % 4 == 0, "%s: pool or table is not aligned to its elements", op );
+  GH_REQUIRE( (uint64_t)p->table_stride * p->page_tokens < 1ull << 31, "%s: a table that reaches 2^31 tokens", op );
+  *out = { static_cast<const char*>( p->pool ), p->page_stride, p->n_pages - 1, (uint32_t)__builtin_ctz( p->page_tokens ), p->table, p->table_stride,
+           (uint32_t)( 2 * kv_dim * size ) };
+  return GH_OK;
+}
+
+// ---- packed sequences ---------------------------------------------------------------------------
+struct Packed
+{
+  const uint32_t* first; // batch + 1
+  const uint32_t* start; // batch, or NULL: all 0
+  uint32_t batch;
+  uint32_t tokens; // rows there are, whatever `first` says
+
+  __device__ __forceinline__ uint32_t begin( uint32_t i ) const { return min( first[i], tokens ); }
+  __device__ __forceinline__ uint32_t count( uint32_t i ) const
+  {
+    const uint32_t b = begin( i ), e = begin( i + 1 );
+    return e > b ? e - b : 0;
+  }
+};
+
+__device__ __forceinline__ uint32_t wave_sum_u32( uint32_t v )
+{
+#pragma unroll
+  for ( int off = 32; off > 0; off >>= 1 ) {
+    v += __shfl_xor( v, off, WAVE );
+  }
+  return v;
+}
+
+// Block number -> (sequence, block of the sequence), by a whole wave.  A sequence of n tokens with `gqa` columns each has ceil(n gqa / columns) blocks; blocks
+// are numbered by falling position in their sequence, so that the ones with the most keys come first and a launch does not end on a long one.  The level (position) of
+// a number is found by bisection over how many blocks lie at a level and above, a sum over the sequences.  False: no such block.
+__device__ __forceinline__ bool packed_block( const Packed& s, uint32_t gqa, uint32_t columns, uint32_t number, uint32_t* seq, uint32_t* block )
+{
+  const uint32_t lane = threadIdx.x & 63;
+  auto blocks = [&]( uint32_t i ) { return i < s.batch ? (uint32_t)( ( (uint64_t)s.count( i ) * gqa + columns - 1 ) / columns ) : 0u; };
+  const uint32_t mine = blocks( lane ); // those of the first 64 sequences are kept
+  uint32_t most = mine;
+  for ( uint32_t i = 64 + lane; i < s.batch; i += 64 ) {
+    most = max( most, blocks( i ) );
+  }
+#pragma unroll
+  for ( int off = 32; off > 0; off >>= 1 ) {
+    most = max( most, __shfl_xor( most, off, WAVE ) );
+  }
+  auto above = [&]( uint32_t level ) { // blocks at `level` and beyond
+    uint32_t n = mine > level ? mine - level : 0;
+    for ( uint32_t i = 64 + lane; i < s.batch; i += 64 ) {
+      const uint32_t b = blocks( i );
+      n += b > level ? b - level : 0;
+    }
+    return wave_sum_u32( n );
+  };
+  if ( above( 0 ) <= number ) {
+    return false;
+  }
+  uint32_t low = 0, high = most; // above( low ) > number >= above( high )
+  while ( high - low > 1 ) {
+    const uint32_t middle = ( low + high ) / 2;
+    if ( above( middle ) > number ) {
+      low = middle;
+    } else {
+      high = middle;
+    }
+  }
+  uint32_t rank = number - above( low + 1 ); // among the sequences that have a block at this level
+  for ( uint32_t i0 = 0; i0 < s.batch; i0 += 64 ) {
+    const uint64_t have = __builtin_amdgcn_ballot_w64( ( i0 == 0 ? mine : blocks( i0 + lane ) ) > low );
+    const uint32_t n = __popcll( have );
+    if ( rank < n ) {
+      // the lane whose set bit has `rank` set bits below it
+      const uint64_t hit = __builtin_amdgcn_ballot_w64( ( have >> lane & 1 ) && (uint32_t)__popcll( have & ( ( 1ull << lane ) - 1 ) ) == rank );
+      *seq = __builtin_amdgcn_readfirstlane( i0 + (uint32_t)__builtin_ctzll( hit ) );
+      *block = __builtin_amdgcn_readfirstlane( low );
+      return true;
+    }
+    rank -= n;
+  }
+  return false;
+}
+
+// The sequence a packed row belongs to, by a whole wave: as many sequences as end at or before it lie in front.  batch: none.
+__device__ __forceinline__ uint32_t packed_sequence( const Packed& s, uint32_t row )
+{
+  uint32_t n = 0;
+  for ( uint32_t i0 = 0; i0 < s.batch; i0 += 64 ) {
+    const uint32_t i = i0 + ( threadIdx.x & 63 );
+    n += __popcll( __builtin_amdgcn_ballot_w64( i < s.batch && s.begin( i + 1 ) <= row ) );
+  }
+  return n < s.batch && s.begin( n ) <= row ? n : s.batch;
+}
+
+// ---- one query row by one wave, key after key -----------------------------------------------------
+// The slow form of an attention over the keys [k0, k1): scores by lanes, 64 keys at a time, then the values one by one, so that only rows that
+// are attended are touched.  The tile kernels take it for rows whose result holds a NaN: a tile multiplies the values behind a token's position by
+// a weight of zero, which makes a NaN of an infinity or a NaN there.  acc[u]: dim 64 u + lane; l is the whole sum.
+template<typename T>
+__device__ __noinline__ void walk_row( const T* q, Pages p, uint32_t seq, uint32_t kv_offset, uint32_t v_offset, uint32_t size, uint32_t k0, uint32_t k1, float scale_log2e,
+                                       float* m_out, float* l_out, float* acc )
+{
+  const uint32_t lane = threadIdx.x & 63;
+  float m = -INFINITY, l = 0.0f;
+  for ( int u = 0; u < 4; u++ ) {
+    acc[u] = 0.0f;
+  }
+  for ( uint32_t key = k0; key < k1; key += 64 ) {
+    float s = -INFINITY;
+    const T* k = reinterpret_cast<const T*>( p.row( seq, min( key + lane, k1 - 1 ) ) ) + kv_offset;
+    float dot = 0.0f;
+    for ( uint32_t d = 0; d < size; d++ ) {
+      dot = __builtin_fmaf( to_f32( q[d] ), to_f32( k[d] ), dot );
+    }
+    if ( key + lane < k1 ) {
+      s = dot * scale_log2e;
+    }
+    const float m_new = fmaxf( m, wave_max( s ) );
+    const float m_safe = m_new == -INFINITY ? 0.0f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f( m - m_safe ), w = __builtin_amdgcn_exp2f( s - m_safe );
+    m = m_new;
+    l = l * alpha + wave_sum( w );
+    for ( int u = 0; u < 4; u++ ) {
+      acc[u] *= alpha;
+    }
+    const uint32_t n = min( 64u, k1 - key );
+    for ( uint32_t j = 0; j < n; j++ ) {
+      const float wj = __shfl( w, (int)j, WAVE );
+      const T* v = reinterpret_cast<const T*>( p.row( seq, key + j ) ) + v_offset;
+      for ( int u = 0; u < 4; u++ ) {
+        const uint32_t d = 64 * u + lane;
+        if ( d < size ) {
+          acc[u] = __builtin_fmaf( wj, to_f32( v[d] ), acc[u] );
+        }
+      }
+    }
+  }
+  *m_out = m;
+  *l_out = l;
+}
+
+} // namespace gh

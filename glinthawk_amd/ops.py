@@ -12,7 +12,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import (GH_ACT_GELU_TANH, GH_ACT_SILU, GH_ATTN_AUTO, GH_BF16, GH_F16, GH_F32, GhMlstm, GhStreamStep, GhUnitHeads, GhWindowAttn, Shape, check,
+from ._lib import (GH_ACT_GELU_TANH, GH_ACT_SILU, GH_ATTN_AUTO, GH_BF16, GH_F16, GH_F32, GhMlstm, GhPages, GhStreamStep, GhUnitHeads, GhWindowAttn, Shape, check,
                    lib)
 
 
@@ -423,6 +423,140 @@ def convert_and_copy(dst, src, n: int, kind: int) -> None:
 
 def convert(dst: torch.Tensor, src: torch.Tensor, n: int) -> None:
     check(lib().gh_convert(_p(dst), _dt(dst), _p(src), _dt(src), n, _stream()), "gh_convert")
+
+
+# ---- a cache in pages -----------------------------------------------------------------------------
+def _same_device(device, **tensors) -> None:
+    """An op's tensors lie on one device, the library's and the current one: a launch on another could not reach them."""
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+def _u32(t: Optional[torch.Tensor], name: str, *shape) -> None:
+    if t is None:
+        return
+    if t.dtype != torch.int32 or not t.is_contiguous() or (shape and tuple(t.shape) != shape):
+        raise ValueError(f"{name}: a contiguous int32 tensor{' of shape ' + str(shape) if shape else ''} expected, got {tuple(t.shape)} of {t.dtype}")
+
+
+def pages(pool: torch.Tensor, table: torch.Tensor) -> GhPages:
+    """pool: (pages, tokens of a page, 2 * kv_dim) of one layer, its pages as far apart as they like; table: (contexts, entries) int32.  Both are kept alive."""
+    if pool.dim() != 3 or pool.stride(2) != 1 or pool.stride(1) != pool.shape[2]:
+        raise ValueError("the rows of a page lie one behind the other: (pages, tokens, 2 * kv_dim) expected")
+    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous():
+        raise ValueError("the table is a contiguous (contexts, entries) int32 tensor")
+    _same_device(pool.device, table=table)
+    p = GhPages(pool.data_ptr(), pool.stride(0) * pool.element_size(), pool.shape[0], pool.shape[1], table.data_ptr(), table.shape[1])
+    p.tensors = (pool, table)
+    return p
+
+
+def _check_paged(p: GhPages, shape: Shape, batch: int, **tensors) -> None:
+    pool, table = p.tensors
+    if pool.shape[2] != 2 * shape.kv_dim:
+        raise ValueError(f"rows of {pool.shape[2]} elements, the shape's have {2 * shape.kv_dim}")
+    if table.shape[0] < batch:
+        raise ValueError(f"a table of {table.shape[0]} contexts for a batch of {batch}")
+    _same_device(pool.device, **tensors)
+    for name in ("q", "xb"):
+        t = tensors[name]
+        if t.dtype != pool.dtype or t.dim() != 2 or t.shape[1] != shape.dim or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous rows of {shape.dim} x {pool.dtype} expected, got {tuple(t.shape)} of {t.dtype}")
+    if tensors["q"].shape != tensors["xb"].shape:
+        raise ValueError("q and xb differ in shape")
+
+
+def page_rows(p: GhPages, first: torch.Tensor, start_pos: Optional[torch.Tensor], n_tokens: int):
+    """(addresses of the tokens' cache rows, their positions): the tables kv_append, rope and matmul_qkv_rope_append take."""
+    pool, table = p.tensors
+    batch = first.numel() - 1
+    _u32(first, "first")
+    _u32(start_pos, "start_pos", batch)
+    if table.shape[0] < batch:
+        raise ValueError(f"a table of {table.shape[0]} contexts for {batch} sequences")
+    _same_device(pool.device, first=first, start_pos=start_pos)
+    rows = torch.empty(n_tokens, dtype=torch.int64, device=pool.device)
+    pos = torch.empty(n_tokens, dtype=torch.int32, device=pool.device)
+    check(lib().gh_page_rows(C.byref(p), _p(first), _p(start_pos), batch, n_tokens, pool.shape[2] // 2, _p(rows), _p(pos), _dt(pool), _stream()), "gh_page_rows")
+    return rows, pos
+
+
+def attn_decode_paged_workspace(batch: int, max_length: int, shape: Shape, dtype: torch.dtype) -> int:
+    s = shape.c()
+    return int(lib().gh_attn_decode_paged_workspace(batch, max_length, C.byref(s), _dt(torch.empty(0, dtype=dtype))))
+
+
+def attn_decode_paged(q: torch.Tensor, p: GhPages, lengths: torch.Tensor, xb: torch.Tensor, max_length: int, shape: Shape,
+                      workspace: Optional[torch.Tensor] = None) -> None:
+    s = shape.c()
+    batch = q.shape[0]
+    _u32(lengths, "lengths", batch)
+    _check_paged(p, shape, batch, q=q, xb=xb, lengths=lengths, workspace=workspace)
+    if workspace is None:
+        workspace = torch.empty(attn_decode_paged_workspace(batch, max_length, shape, q.dtype), dtype=torch.uint8, device=q.device)
+    check(lib().gh_attn_decode_paged(_p(q), C.byref(p), _p(lengths), _p(xb), batch, max_length, C.byref(s), _dt(q), _p(workspace),
+                                     workspace.numel() * workspace.element_size(), _stream()), "gh_attn_decode_paged")
+
+
+def attn_packed_workspace(batch: int, n_tokens: int, max_keys: int, shape: Shape, dtype: torch.dtype) -> int:
+    s = shape.c()
+    return int(lib().gh_attn_packed_workspace(batch, n_tokens, max_keys, C.byref(s), _dt(torch.empty(0, dtype=dtype))))
+
+
+def attn_packed(q: torch.Tensor, p: GhPages, first: torch.Tensor, start_pos: Optional[torch.Tensor], xb: torch.Tensor, max_keys: int, shape: Shape,
+                workspace: Optional[torch.Tensor] = None) -> None:
+    """first: (sequences + 1) int32, where each sequence's tokens begin in q and xb; start_pos: (sequences) int32 or None."""
+    s = shape.c()
+    batch = first.numel() - 1
+    _u32(first, "first")
+    _u32(start_pos, "start_pos", batch)
+    _check_paged(p, shape, batch, q=q, xb=xb, first=first, start_pos=start_pos, workspace=workspace)
+    if workspace is None:
+        workspace = torch.empty(attn_packed_workspace(batch, q.shape[0], max_keys, shape, q.dtype), dtype=torch.uint8, device=q.device)
+    check(lib().gh_attn_packed(_p(q), C.byref(p), _p(first), _p(start_pos), _p(xb), batch, q.shape[0], max_keys, C.byref(s), _dt(q), _p(workspace),
+                               workspace.numel() * workspace.element_size(), _stream()), "gh_attn_packed")
+
+
+def copy_pages(pool: torch.Tensor, pairs) -> None:
+    """pool: (layers, pages, tokens, elements) or (pages, tokens, elements); pairs: (n, 2) of (source, destination), an int32 tensor on the device or a
+    sequence of pairs in host memory, which is checked."""
+    layered = pool if pool.dim() == 4 else pool[None]
+    if layered.dim() != 4 or layered.stride(3) != 1 or layered.stride(2) != layered.shape[3]:
+        raise ValueError("the rows of a page lie one behind the other: ([layers,] pages, tokens, elements) expected")
+    size = pool.element_size()
+    layers, n_pages, tokens, row = layered.shape
+    common = layered.data_ptr(), layered.stride(1) * size, tokens * row * size, n_pages, layers, layered.stride(0) * size
+    if isinstance(pairs, torch.Tensor):
+        if pairs.dim() != 2 or pairs.shape[1] != 2:
+            raise ValueError(f"pairs: (n, 2) expected, got {tuple(pairs.shape)}")
+        _u32(pairs, "pairs")
+        _same_device(pool.device, pairs=pairs)
+        check(lib().gh_copy_pages(*common, _p(pairs), pairs.shape[0], _stream()), "gh_copy_pages")
+    else:
+        flat = [int(v) for pair in pairs for v in pair]
+        check(lib().gh_copy_pages_host(*common, host_u32_array(flat), len(flat) // 2, _stream()), "gh_copy_pages_host")
+
+
+def token_logprobs_workspace(rows: int, vocab: int, n_top: int) -> int:
+    return int(lib().gh_token_logprobs_workspace(rows, vocab, n_top))
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, n_top: int = 0, workspace: Optional[torch.Tensor] = None):
+    """(log probability of each row's token, entropy, (rows, n_top) indices of the largest values, their log probabilities)"""
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("rows of logits lie with their values one behind the other")
+    rows, vocab = logits.shape
+    _u32(tokens, "tokens", rows)
+    _same_device(logits.device, tokens=tokens, workspace=workspace)
+    if workspace is None:
+        workspace = torch.empty(token_logprobs_workspace(rows, vocab, n_top), dtype=torch.uint8, device=logits.device)
+    given, entropy = torch.empty((2, rows), dtype=torch.float32, device=logits.device).unbind()
+    ids = torch.empty((rows, n_top), dtype=torch.int32, device=logits.device)
+    values = torch.empty((rows, n_top), dtype=torch.float32, device=logits.device)
+    check(lib().gh_token_logprobs(_p(given), _p(entropy), _p(ids), _p(values), logits.data_ptr(), logits.stride(0), _p(tokens), vocab, rows, n_top, _dt(logits),
+                                  _p(workspace), workspace.numel() * workspace.element_size(), _stream()), "gh_token_logprobs")
+    return given, entropy, ids, values
 
 
 # ---- run-time sized designs -----------------------------------------------------------------------

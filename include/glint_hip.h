@@ -41,7 +41,7 @@ typedef enum gh_dtype
 {
   GH_F16 = 0,
   GH_F32 = 1,
-  GH_BF16 = 2 /* the dense products and the ops of the run-time sized designs below; the Llama2 ops refuse it (the reference's amd64 bf16 is an alias of fp16, arch/float.hh:13) */
+  GH_BF16 = 2 /* the dense products, the cache in pages with gh_kv_append and gh_rope, gh_token_logprobs and the ops of the run-time sized designs below; the other Llama2 ops refuse it (the reference's amd64 bf16 is an alias of fp16, arch/float.hh:13) */
 } gh_dtype;
 
 /* values equal glinthawk::CopyType (models/types.hh:127-133) */
@@ -371,6 +371,56 @@ uint64_t gh_attn_prefill_workspace( uint64_t batch, uint32_t n_tokens, const gh_
 int gh_attn_set_prefill_tiles( int column_tiles_per_wave );
 int gh_attn_prefill( const void* q, const void* const* layer_rows_dev, const uint32_t* start_pos_dev, void* xb, uint64_t batch, uint32_t n_tokens,
                      uint32_t max_start_pos, const gh_shape* shape, gh_dtype dt, void* workspace, uint64_t workspace_bytes, int variant, gh_stream stream );
+
+/* ---- a cache in pages -------------------------------------------------------------------------------
+ * No counterpart in the reference, whose contexts are one run of rows each.  A layer's cache is a pool of pages, a page page_tokens rows
+ * [K | V] one behind the other, and every context (or sequence) has a line of page numbers in `table`: its token t lies in row
+ * t % page_tokens of page table[context * table_stride + t / page_tokens].  Contexts may have pages in common.  A page number that is not
+ * below n_pages reads as the last page: nothing outside the pool is touched, and what such a context gives is not specified.
+ * Storage types f16, bf16 and f32; K, V and queries alike.  Head sizes up to 256, any gqa. */
+typedef struct gh_pages
+{
+  void* pool;               /* this layer's pages; page p begins p * page_stride bytes from here; aligned to its elements */
+  uint64_t page_stride;     /* at least page_tokens * 2 * kv_dim elements, a multiple of the element size */
+  uint32_t n_pages;
+  uint32_t page_tokens;     /* a power of two; a page below 2 GiB */
+  const uint32_t* table;    /* device memory, (batch, table_stride) */
+  uint32_t table_stride;    /* tokens of a context that the table reaches: table_stride * page_tokens, below 2^31 */
+} gh_pages;
+/* Cache rows and positions of the new tokens of packed sequences: tokens [first_dev[i], first_dev[i + 1]) belong to sequence i and stand at positions
+ * start_pos_dev[i] and up (start_pos_dev NULL: all 0).  token_rows_out and pos_out (n_tokens each, either may be NULL) are the tables that gh_kv_append,
+ * gh_rope and the fused projections take.  A token that no sequence has, or whose position the table does not reach, or whose page number is not below
+ * n_pages gets a NULL row, which those ops skip. */
+int gh_page_rows( const gh_pages* pages, const uint32_t* first_dev, const uint32_t* start_pos_dev, uint64_t batch, uint64_t n_tokens, uint32_t kv_dim,
+                  void** token_rows_out, uint32_t* pos_out, gh_dtype dt, gh_stream stream );
+/* gh_attn_decode over pages: query row i attends the keys [0, lengths_dev[i]) of context i, the current token's among them.  Length 0: an empty context,
+ * whose row of xb is left as it is.  max_length: host-side upper bound of the lengths (at most what the table reaches); keys beyond it are not attended.
+ * The workspace (gh_attn_decode_paged_workspace, 0 bytes where the call needs none; 16-byte aligned) is for this call alone while it runs: calls that may
+ * overlap in time, graphs that were captured with it among them, take one each.  The shape's seq_len is not looked at. */
+uint64_t gh_attn_decode_paged_workspace( uint64_t batch, uint32_t max_length, const gh_shape* shape, gh_dtype dt );
+int gh_attn_decode_paged( const void* q, const gh_pages* pages, const uint32_t* lengths_dev, void* xb, uint64_t batch, uint32_t max_length, const gh_shape* shape,
+                          gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream );
+/* Causal attention of packed prompts over pages, their rows already appended and rotated: tokens [first_dev[i], first_dev[i + 1]) are new tokens of sequence i
+ * at positions start_pos_dev[i] and up (NULL: all 0), and each attends the keys up to its own position.  A sequence may have no tokens.  q and xb are
+ * (n_tokens, dim); rows that no sequence has are left as they are.  max_keys: host-side upper bound of start position + tokens (at most what the table reaches);
+ * a sequence that goes beyond it attends no keys from there on.  Values behind a token's own position do not reach its output, whatever they are.  Workspace as above. */
+uint64_t gh_attn_packed_workspace( uint64_t batch, uint64_t n_tokens, uint32_t max_keys, const gh_shape* shape, gh_dtype dt );
+int gh_attn_packed( const void* q, const gh_pages* pages, const uint32_t* first_dev, const uint32_t* start_pos_dev, void* xb, uint64_t batch, uint64_t n_tokens,
+                    uint32_t max_keys, const gh_shape* shape, gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream );
+/* Pages copied within a pool, in each of `layers` layers (layer k's pages begin layer_stride bytes behind those of k - 1): page pairs[2 j + 1] becomes a copy of
+ * page pairs[2 j], page_bytes bytes of it.  A pair with a number that is not below n_pages is left out.  No page may be written twice, or be both written and read, in
+ * one call: the host form checks it, and the numbers, and refuses; the plain form's pairs are in device memory and are the caller's to keep apart. */
+int gh_copy_pages( void* pool, uint64_t page_stride, uint64_t page_bytes, uint32_t n_pages, uint64_t layers, uint64_t layer_stride, const uint32_t* pairs_dev,
+                   uint64_t n_pairs, gh_stream stream );
+int gh_copy_pages_host( void* pool, uint64_t page_stride, uint64_t page_bytes, uint32_t n_pages, uint64_t layers, uint64_t layer_stride, const uint32_t* pairs_host,
+                        uint64_t n_pairs, gh_stream stream );
+/* What a caller asks of rows of logits besides gh_argmax: with p = softmax(row), fp32 results
+ *   logprob(i) = ln p[tokens_dev[i]] (left as it is where the token is not below vocab);  entropy(i) = - sum p ln p, a value of -inf counting as none;
+ *   top_ids, top_logprobs (rows, n_top) = the n_top largest values of the row, largest first, the lower index first among equals, NaN behind everything.
+ * logprob with tokens_dev, entropy, and the two of the alternatives may be NULL where they are not wanted (n_top 0).  Rows lie row_stride elements apart; n_top up to 64. */
+uint64_t gh_token_logprobs_workspace( uint64_t rows, uint64_t vocab, uint32_t n_top );
+int gh_token_logprobs( float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs, const void* logits, uint64_t row_stride, const uint32_t* tokens_dev,
+                       uint64_t vocab, uint64_t rows, uint32_t n_top, gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream );
 
 /* ---- designs whose sizes come at run time ---------------------------------------------------------
  * Ops of decoder-only designs beyond Llama2 (no counterpart in the reference): storage type GH_BF16 or GH_F32, the residual stream x,
