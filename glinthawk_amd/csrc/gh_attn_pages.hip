@@ -70,6 +70,30 @@ __device__ __forceinline__ bool block_of( const Call& a, uint32_t number, uint32
 // keys that token t of a block's sequence attends
 __device__ __forceinline__ uint32_t visible( const Call& a, const Block& b, uint32_t t ) { return min( b.start + t + 1, a.max_keys ); }
 
+// A column (by its number in the sequence) of a tile kernel's split once more, by a whole wave, with its result put where the tile's would be.
+template<typename T>
+__device__ __noinline__ void walk_column( const T* q, T* out, Call a, Block b, uint32_t col, uint32_t k_begin, uint32_t k_end )
+{
+  const uint32_t lane = threadIdx.x & 63;
+  const uint64_t place = (uint64_t)( b.row0 + col / a.gqa ) * a.n_kv_heads * a.gqa + b.h * a.gqa + col % a.gqa, slot = place * a.splits + b.split;
+  float m, l, acc[4];
+  walk_row<T>( q + place * a.size, a.pages, b.seq, b.h * a.size, ( a.n_kv_heads + b.h ) * a.size, a.size, k_begin, k_end, a.scale_log2e, &m, &l, acc );
+  for ( uint32_t u = 0; u < 4; u++ ) {
+    const uint32_t d = 64 * u + lane;
+    if ( d < a.size ) {
+      if ( a.splits == 1 ) {
+        out[place * a.size + d] = from_f32<T>( acc[u] / l );
+      } else {
+        a.part_out[slot * a.size + d] = acc[u];
+      }
+    }
+  }
+  if ( a.splits > 1 && lane == 0 ) {
+    a.part_ml[slot * 2] = m;
+    a.part_ml[slot * 2 + 1] = l;
+  }
+}
+
 template<typename T>
 struct alignas( 4 * sizeof( T ) ) Piece
 {
@@ -284,28 +308,9 @@ __global__ __launch_bounds__( 256 ) void attn_pages_f32_kernel( const T* __restr
     todo = ( todo | todo >> 16 | todo >> 32 | todo >> 48 ) & 0xffff; // columns
     if ( todo != 0 ) {
       const uint32_t keep = ok && !( todo >> c & 1 );
-      for ( uint32_t cc = 0; cc < 16; cc++ ) {
-        if ( !( todo >> cc & 1 ) ) {
-          continue;
-        }
-        const uint32_t cl = b.col0 + 16 * wave + cc, t = cl / a.gqa, hd = b.h * a.gqa + cl % a.gqa;
-        const uint64_t at = (uint64_t)( b.row0 + t ) * n_heads + hd;
-        float wm, wl, wacc[4];
-        walk_row<T>( q + at * a.size, a.pages, b.seq, kv_off, v_off, a.size, k_begin, min( visible( a, b, t ), k_end ), a.scale_log2e, &wm, &wl, wacc );
-        for ( int u = 0; u < 4; u++ ) {
-          const uint32_t d = 64 * u + lane;
-          if ( d < a.size ) {
-            if ( a.splits == 1 ) {
-              out[at * a.size + d] = from_f32<T>( wacc[u] / wl );
-            } else {
-              a.part_out[( at * a.splits + b.split ) * a.size + d] = wacc[u];
-            }
-          }
-        }
-        if ( a.splits > 1 && lane == 0 ) {
-          a.part_ml[( at * a.splits + b.split ) * 2] = wm;
-          a.part_ml[( at * a.splits + b.split ) * 2 + 1] = wl;
-        }
+      for ( ; todo != 0; todo &= todo - 1 ) {
+        const uint32_t cl = b.col0 + 16 * wave + (uint32_t)__builtin_ctzll( todo );
+        walk_column<T>( q, out, a, b, cl, k_begin, min( visible( a, b, cl / a.gqa ), k_end ) );
       }
       if ( !keep ) {
         return;
@@ -357,32 +362,698 @@ __global__ __launch_bounds__( 256 ) void attn_pages_f32_kernel( const T* __restr
 }
 
 // =================================================================================================
-// splits of a row added up: wave <-> (query row, head)
+// decode, 16-bit heads of 8 CH elements and fewer: wave <-> (context, kv head, 16 columns, run of keys)
+//
+// Bound by the bytes of the cache.  A wave goes through stages of 32 keys on its own: their K and V rows go from memory straight to its part of LDS, two stages deep,
+// so that a stage (16 KB at 128 elements) is always on its way while one is computed.  Rows behind the keys, and chunks behind a smaller head, lie outside the
+// descriptor of their 16 rows (which lie in one page) and arrive as zeros, whatever memory holds there.
+//   S^T = K Q^T     16 x 16 x 32: a lane gets keys 4 g + i (and 16 + 4 g + i) of column c
+//   O^T += V^T P^T  16 x 16 x 32: the weights are the second operand as they lie, if slot 8 g + e is key 4 g + e (e < 4) and 16 + 4 g + e - 4; the first operand's
+//                   lanes take those keys of one dim with transposing LDS reads
+// 16-byte chunks of a row are swizzled by the row (in the address a lane fetches) so that both reads touch every bank once.
+// The weights are rounded to the storage type for the second product, as the matrix units take them; the sum takes them rounded too.
+// W waves of a work-group take the stages of one run in turns and are joined through LDS.
 // =================================================================================================
-template<typename T, bool DECODE>
-__global__ __launch_bounds__( 256 ) void pages_merge_kernel( T* __restrict__ out, Call a, uint32_t rows )
+typedef __attribute__( ( address_space( 3 ) ) ) void* lds_ptr;
+typedef __attribute__( ( address_space( 3 ) ) ) char lds_char;
+typedef short v4s __attribute__( ( ext_vector_type( 4 ) ) );
+typedef short v8s __attribute__( ( ext_vector_type( 8 ) ) );
+typedef __attribute__( ( address_space( 3 ) ) ) v4s* lds_v4s;
+
+constexpr float LAZY = 8.0f; // the reference point of the exponentials stays until a maximum is 2^LAZY above it: weights up to 256, fewer rescalings
+
+// maximum over the lanes that share a column, 16 lanes apart, without a trip through LDS
+__device__ __forceinline__ float column_max( float v )
 {
-  const uint32_t lane = threadIdx.x & 63, n_heads = a.n_kv_heads * a.gqa;
-  const uint64_t place = (uint64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 );
-  const uint32_t row = (uint32_t)( place / n_heads );
-  if ( row >= rows ) {
+  v = half_wave_max( v );
+  const unsigned bits = __builtin_bit_cast( unsigned, v );
+  const auto r = __builtin_amdgcn_permlane16_swap( bits, bits, false, false );
+  const unsigned r0 = r[0], r1 = r[1];
+  return fmaxf( __builtin_bit_cast( float, r0 ), __builtin_bit_cast( float, r1 ) );
+}
+__device__ __forceinline__ float column_sum( float v ) { return sum_rows( sum_halves( v, v ), sum_halves( v, v ) ); }
+
+// a weight as the storage type holds it
+template<typename E>
+__device__ __forceinline__ float rounded( float v )
+{
+  return to_f32( from_f32<E>( v ) );
+}
+
+// LDS reads of a stage, written out, each block with its waits: the compiler cannot tell the tiles that a read may take from the ones on their way, and would wait
+// for all of them.
+template<int CH, uint32_t FIRST, uint32_t SECOND, typename X8>
+__device__ __forceinline__ void read_keys( const uint32_t* at, X8 ( &k )[2][CH / 4] )
+{
+  if constexpr ( CH == 16 ) {
+    asm volatile( "s_waitcnt vmcnt(16)\n\t"
+                  "ds_read_b128 %0, %8 offset:%12\n\t"
+                  "ds_read_b128 %1, %9 offset:%12\n\t"
+                  "ds_read_b128 %2, %10 offset:%12\n\t"
+                  "ds_read_b128 %3, %11 offset:%12\n\t"
+                  "ds_read_b128 %4, %8 offset:%13\n\t"
+                  "ds_read_b128 %5, %9 offset:%13\n\t"
+                  "ds_read_b128 %6, %10 offset:%13\n\t"
+                  "ds_read_b128 %7, %11 offset:%13\n\t"
+                  "s_waitcnt lgkmcnt(0)"
+                  : "=&v"( k[0][0] ), "=&v"( k[0][1] ), "=&v"( k[0][2] ), "=&v"( k[0][3] ), "=&v"( k[1][0] ), "=&v"( k[1][1] ), "=&v"( k[1][2] ), "=&v"( k[1][3] )
+                  : "v"( at[0] ), "v"( at[1] ), "v"( at[2] ), "v"( at[3] ), "n"( FIRST ), "n"( SECOND )
+                  : "memory" );
+  } else {
+    asm volatile( "s_waitcnt vmcnt(8)\n\t"
+                  "ds_read_b128 %0, %4 offset:%6\n\t"
+                  "ds_read_b128 %1, %5 offset:%6\n\t"
+                  "ds_read_b128 %2, %4 offset:%7\n\t"
+                  "ds_read_b128 %3, %5 offset:%7\n\t"
+                  "s_waitcnt lgkmcnt(0)"
+                  : "=&v"( k[0][0] ), "=&v"( k[0][1] ), "=&v"( k[1][0] ), "=&v"( k[1][1] )
+                  : "v"( at[0] ), "v"( at[1] ), "n"( FIRST ), "n"( SECOND )
+                  : "memory" );
+  }
+}
+// four blocks of 16 dims
+template<uint32_t FIRST, uint32_t SECOND>
+__device__ __forceinline__ void read_values( const uint32_t* at, v4s ( *v )[2] )
+{
+  asm volatile( "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+                "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+                "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+                "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+                "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"( v[0][0] ), "=&v"( v[0][1] ), "=&v"( v[1][0] ), "=&v"( v[1][1] ), "=&v"( v[2][0] ), "=&v"( v[2][1] ), "=&v"( v[3][0] ), "=&v"( v[3][1] )
+                : "v"( at[0] ), "v"( at[1] ), "v"( at[2] ), "v"( at[3] ), "n"( FIRST ), "n"( SECOND )
+                : "memory" );
+}
+
+template<typename E, int CH, int W, int HW>
+__device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restrict__ out, const Call& a )
+{
+  constexpr uint32_t KK = CH / 4, NB = CH / 2; // k steps of the scores, blocks of 16 dims
+  constexpr uint32_t RPI = 64 / CH;            // rows that a load of the wave fetches
+  constexpr uint32_t IPG = 16 / RPI;           // loads for 16 rows of K, or of V
+  using X8 = typename Mfma<E>::x8;
+  constexpr uint32_t TILE = 32 * CH * 16;      // bytes
+  static_assert( W == 1 || HW == 1, "" );
+  __shared__ uint4 s_tiles[W * HW][4][32 * CH]; // of every wave: K of even and of odd stages, V of even and of odd stages
+
+  const uint32_t wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 ), lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
+  Block b;
+  const uint32_t pairs = a.n_kv_heads / HW, hw = HW == 1 ? 0 : __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 );
+  if ( !block_of<true, 16>( a, blockIdx.x / pairs, blockIdx.x % pairs * HW + hw, blockIdx.y, &b ) ) {
     return;
   }
-  uint32_t keys;
-  if constexpr ( DECODE ) {
-    keys = min( a.lengths[row], a.max_keys );
-  } else {
-    const uint32_t seq = packed_sequence( a.seqs, row );
-    if ( seq >= a.seqs.batch || a.seqs.count( seq ) <= row - a.seqs.begin( seq ) ) {
+  const uint32_t length = b.start + 1, k_begin = b.split * a.chunk, k_end = min( length, k_begin + a.chunk );
+  if ( k_begin >= k_end ) {
+    return;
+  }
+  const uint32_t col = b.col0 + c;
+  const bool ok = col < a.gqa;
+  const uint64_t place = (uint64_t)b.row0 * a.n_kv_heads * a.gqa + (uint64_t)b.h * a.gqa + ( ok ? col : 0 );
+
+  uint4( *const tiles )[32 * CH] = s_tiles[wave + hw];
+  X8 qb[KK];
+#pragma unroll
+  for ( uint32_t kk = 0; kk < KK; kk++ ) {
+    const uint32_t d = 8 * ( 4 * kk + g4 );
+    qb[kk] = ok && d < a.size ? *reinterpret_cast<const X8*>( q + place * a.size + d ) : X8 { 0, 0, 0, 0, 0, 0, 0, 0 };
+  }
+
+  // a lane's place in the rows of a load: row lane / CH, slot lane % CH, which keeps chunk slot ^ (swizzle of the row)
+  const uint32_t ld_row = lane / CH, ld_slot = lane % CH, chunks = a.size / 8;
+  const uint32_t k_off = b.h * a.size * 2, v_off = ( a.n_kv_heads + b.h ) * a.size * 2;
+  auto k_swizzle = []( uint32_t row ) { return CH == 16 ? row & 15 : ( row >> 1 ) & 7; };
+  auto v_swizzle = []( uint32_t row ) { return CH == 16 ? 2 * ( row & 7 ) : 2 * ( ( row >> 1 ) & 3 ); };
+  uint32_t k_at[IPG], v_at[IPG];
+#pragma unroll
+  for ( uint32_t t = 0; t < IPG; t++ ) {
+    const uint32_t row = RPI * t + ld_row, kc = ld_slot ^ k_swizzle( row ), vc = ld_slot ^ v_swizzle( row );
+    k_at[t] = kc < chunks ? row * a.pages.row_bytes + k_off + 16 * kc : 0x80000000u; // far outside every descriptor
+    v_at[t] = vc < chunks ? row * a.pages.row_bytes + v_off + 16 * vc : 0x80000000u;
+  }
+
+  const uint32_t n_stages = ( k_end - k_begin + 31 ) / 32, n_mine = n_stages > wave ? ( n_stages - wave + W - 1 ) / W : 0;
+  // Page numbers are read by scalar loads one stage before they are needed: vector loads would be counted with the loads to LDS, and waiting for one would be
+  // waiting for those.
+  typedef const uint32_t __attribute__( ( address_space( 4 ) ) ) * scalar_ptr;
+  const scalar_ptr table = (scalar_ptr)( reinterpret_cast<uintptr_t>( a.pages.table + (uint64_t)b.seq * a.pages.table_stride ) );
+  uint32_t id[2];
+  auto look_up = [&]( uint32_t stage ) __attribute__( ( always_inline ) ) {
+#pragma unroll
+    for ( uint32_t u = 0; u < 2; u++ ) {
+      id[u] = table[min( k_begin + 32 * ( stage * W + wave ) + 16 * u, k_end - 1 ) >> a.pages.shift];
+    }
+  };
+  __amdgpu_buffer_rsrc_t rsrc[2];
+  auto describe = [&]( uint32_t stage ) __attribute__( ( always_inline ) ) {
+#pragma unroll
+    for ( uint32_t u = 0; u < 2; u++ ) {
+      const uint32_t key = k_begin + 32 * ( stage * W + wave ) + 16 * u;
+      const char* base = a.pages.pool + min( id[u], a.pages.last ) * a.pages.stride + (uint64_t)( key & ( ( 1u << a.pages.shift ) - 1 ) ) * a.pages.row_bytes;
+      const uint32_t rows = key < k_end ? min( k_end - key, 16u ) : 0u;
+      rsrc[u] = __builtin_amdgcn_make_buffer_rsrc( const_cast<char*>( base ), 0, (int)( rows * a.pages.row_bytes ), 0x00020000 );
+    }
+    look_up( stage + 1 );
+  };
+  auto fetch = [&]( uint4* tile, const uint32_t( &at )[IPG] ) __attribute__( ( always_inline ) ) {
+#pragma unroll
+    for ( uint32_t u = 0; u < 2; u++ ) {
+#pragma unroll
+      for ( uint32_t t = 0; t < IPG; t++ ) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds( rsrc[u], (lds_ptr)( tile + ( 16 * u + RPI * t ) * CH ), 16, at[t], 0, 0, 2 ); // (read once: streaming)
+      }
+    }
+  };
+
+  mfma_f32x4 acc[NB]; // element i of acc[n]: dim 16 n + 4 g4 + i of column c
+#pragma unroll
+  for ( uint32_t n = 0; n < NB; n++ ) {
+    acc[n] = mfma_f32x4 { 0, 0, 0, 0 };
+  }
+  float m = -INFINITY, l = 0.0f; // l: of this lane's keys
+
+  // K: row c and row 16 + c, chunk 4 kk + g4.  V, transposing: lane 4 e + p of 16 points at dims 4 p .. 4 p + 3 of key 4 g4 + e and receives
+  // one dim of the four keys.
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)&tiles[0][0];
+  const uint32_t tr_row = 4 * g4 + ( c >> 2 ), tr_at = tr_row * CH * 16 + ( ( ( c & 3 ) >> 1 ) ^ v_swizzle( tr_row ) ) * 16 + ( c & 1 ) * 8;
+  uint32_t k_lds[KK], v_lds[NB];
+#pragma unroll
+  for ( uint32_t kk = 0; kk < KK; kk++ ) {
+    k_lds[kk] = lds0 + c * CH * 16 + ( ( 4 * kk + g4 ) ^ k_swizzle( c ) ) * 16;
+  }
+#pragma unroll
+  for ( uint32_t n = 0; n < NB; n++ ) {
+    v_lds[n] = lds0 + ( tr_at ^ ( 32 * n ) );
+  }
+  // buffer: 0 or 1, j % 2
+  auto stage = [&]( uint32_t j, auto buffer ) __attribute__( ( always_inline ) ) {
+    constexpr uint32_t B = decltype( buffer )::value, K0 = B * TILE, K1 = K0 + TILE / 2, V0 = ( 2 + B ) * TILE, V1 = V0 + TILE / 2;
+    uint4* const kt = tiles[B];
+    uint4* const vt = tiles[2 + B];
+    X8 kf[2][KK];
+    read_keys<CH, K0, K1>( k_lds, kf ); // all but the 4 IPG loads of stage j + 1 have landed
+    __builtin_amdgcn_sched_barrier( 0 );
+    describe( j + 2 );
+    fetch( kt, k_at ); // the tile has been read
+    mfma_f32x4 st[2];
+#pragma unroll
+    for ( uint32_t u = 0; u < 2; u++ ) {
+      st[u] = mfma_f32x4 { 0, 0, 0, 0 };
+#pragma unroll
+      for ( uint32_t kk = 0; kk < KK; kk++ ) {
+        st[u] = Mfma<E>::k32( kf[u][kk], qb[kk], st[u] );
+      }
+    }
+    const uint32_t key0 = k_begin + 32 * ( j * W + wave );
+    if ( key0 + 32 > k_end ) {
+#pragma unroll
+      for ( int e = 0; e < 8; e++ ) {
+        st[e >> 2][e & 3] = key0 + 16 * ( e >> 2 ) + 4 * g4 + ( e & 3 ) < k_end ? st[e >> 2][e & 3] : -INFINITY;
+      }
+    }
+    float mx = fmaxf( fmaxf( fmaxf( st[0][0], st[0][1] ), fmaxf( st[0][2], st[0][3] ) ), fmaxf( fmaxf( st[1][0], st[1][1] ), fmaxf( st[1][2], st[1][3] ) ) );
+    mx = column_max( mx ) * a.scale_log2e;
+    if ( __builtin_amdgcn_ballot_w64( mx > m + LAZY ) != 0 ) {
+      const float m_new = fmaxf( m, mx ), alpha = m_new == -INFINITY ? 1.0f : fast_exp2( m - m_new );
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for ( uint32_t n = 0; n < NB; n++ ) {
+        acc[n] *= alpha;
+      }
+    }
+    const float ms = m == -INFINITY ? 0.0f : m;
+    float p[8];
+#pragma unroll
+    for ( int e = 0; e < 8; e++ ) {
+      p[e] = fast_exp2( __builtin_fmaf( st[e >> 2][e & 3], a.scale_log2e, -ms ) );
+    }
+    typedef uint32_t u32x4 __attribute__( ( ext_vector_type( 4 ) ) );
+    const X8 pk = __builtin_bit_cast( X8, ( u32x4 { rounded_pair<E>( p[0], p[1] ), rounded_pair<E>( p[2], p[3] ), rounded_pair<E>( p[4], p[5] ), rounded_pair<E>( p[6], p[7] ) } ) );
+    float sum[2] = { 0, 0 };
+#pragma unroll
+    for ( int e = 0; e < 8; e++ ) {
+      sum[e & 1] += (float)pk[e];
+    }
+    l += sum[0] + sum[1];
+    v4s half[NB][2];
+#pragma unroll
+    for ( uint32_t n = 0; n < NB; n += 4 ) {
+      read_values<V0, V1>( v_lds + n, half + n );
+    }
+    __builtin_amdgcn_sched_barrier( 0 );
+    fetch( vt, v_at );
+    __builtin_amdgcn_sched_barrier( 0 );
+#pragma unroll
+    for ( uint32_t n = 0; n < NB; n++ ) {
+      const v8s v = v8s { half[n][0][0], half[n][0][1], half[n][0][2], half[n][0][3], half[n][1][0], half[n][1][1], half[n][1][2], half[n][1][3] };
+      acc[n] = Mfma<E>::k32( __builtin_bit_cast( X8, v ), pk, acc[n] );
+    }
+  };
+
+  if ( n_mine != 0 ) {
+    look_up( 0 );
+    describe( 0 );
+    fetch( tiles[0], k_at );
+    fetch( tiles[2], v_at );
+    describe( 1 );
+    fetch( tiles[1], k_at );
+    fetch( tiles[3], v_at );
+    for ( uint32_t j = 0; j < n_mine; j += 2 ) { // (loads past the end fetch nothing, so that the count of those on their way stays the same)
+      stage( j, std::integral_constant<uint32_t, 0> {} );
+      if ( j + 1 < n_mine ) {
+        stage( j + 1, std::integral_constant<uint32_t, 1> {} );
+      }
+    }
+  }
+  __builtin_amdgcn_s_waitcnt( 0x0F70 ); // vmcnt(0): nothing is on its way to LDS any more
+  l = column_sum( l );
+
+  if constexpr ( W > 1 ) {
+    // the waves' parts added up by wave 0, lane for lane as they lie in the registers
+    constexpr uint32_t PART = 64 * ( 4 * NB + 2 );
+    static_assert( ( W - 1 ) * PART * 4 <= sizeof( s_tiles ), "the parts fit" );
+    float* parts = reinterpret_cast<float*>( s_tiles );
+    __syncthreads();
+    if ( wave != 0 ) {
+      float* part = parts + ( wave - 1 ) * PART;
+      part[lane] = m;
+      part[64 + lane] = l;
+#pragma unroll
+      for ( uint32_t n = 0; n < NB; n++ ) {
+#pragma unroll
+        for ( int i = 0; i < 4; i++ ) {
+          part[( 2 + 4 * n + i ) * 64 + lane] = acc[n][i];
+        }
+      }
+    }
+    __syncthreads();
+    if ( wave != 0 ) {
       return;
     }
-    const uint32_t start = a.seqs.start ? min( a.seqs.start[seq], 0x7fffffffu ) : 0u;
-    keys = min( start + ( row - a.seqs.begin( seq ) ) + 1, a.max_keys );
+    float mm = m;
+#pragma unroll
+    for ( int w = 0; w < W - 1; w++ ) {
+      mm = fmaxf( mm, parts[w * PART + lane] );
+    }
+    const float mm_safe = mm == -INFINITY ? 0.0f : mm, w0 = fast_exp2( m - mm_safe );
+    m = mm;
+    l *= w0;
+#pragma unroll
+    for ( uint32_t n = 0; n < NB; n++ ) {
+      acc[n] *= w0;
+    }
+#pragma unroll
+    for ( int w = 0; w < W - 1; w++ ) {
+      const float* part = parts + w * PART;
+      const float ww = fast_exp2( part[lane] - mm_safe );
+      l = __builtin_fmaf( part[64 + lane], ww, l );
+#pragma unroll
+      for ( uint32_t n = 0; n < NB; n++ ) {
+#pragma unroll
+        for ( int i = 0; i < 4; i++ ) {
+          acc[n][i] = __builtin_fmaf( part[( 2 + 4 * n + i ) * 64 + lane], ww, acc[n][i] );
+        }
+      }
+    }
   }
-  const uint32_t n = ( keys + a.chunk - 1 ) / a.chunk; // at most a.splits, as max_keys is at most splits * chunk
-  if ( n == 0 ) {
+  if ( !ok ) {
     return;
   }
+  const uint64_t slot = place * a.splits + b.split;
+  const float inv = 1.0f / l;
+#pragma unroll
+  for ( uint32_t n = 0; n < NB; n++ ) {
+    const uint32_t d = 16 * n + 4 * g4;
+    if ( d < a.size ) {
+      if ( a.splits > 1 ) {
+        *reinterpret_cast<mfma_f32x4*>( a.part_out + slot * a.size + d ) = acc[n];
+      } else {
+        *reinterpret_cast<uint2*>( out + place * a.size + d ) = make_uint2( rounded_pair<E>( acc[n][0] * inv, acc[n][1] * inv ), rounded_pair<E>( acc[n][2] * inv, acc[n][3] * inv ) );
+      }
+    }
+  }
+  if ( a.splits > 1 && g4 == 0 ) {
+    a.part_ml[slot * 2] = m;
+    a.part_ml[slot * 2 + 1] = l;
+  }
+}
+
+template<typename E, int CH, int W, int HW>
+__global__ __launch_bounds__( 64 * W * HW ) void attn_pages_decode_kernel( const E* __restrict__ q, E* __restrict__ out, Call a )
+{
+  decode_run<E, CH, W, HW>( q, out, a );
+}
+
+// =================================================================================================
+// packed prompts, 16-bit heads of 8 CH elements and fewer: 128 columns a work-group, 32 a wave, stages of 64 keys
+//
+// Bound by the matrix units where sequences are long.  K and V rows go from memory straight to LDS, two stages of each; a wave fetches 16 rows of a stage, which
+// lie in one page, and rows behind the last key of the work-group, like chunks behind a smaller head, lie outside the descriptor and arrive as zeros.
+//   S^T = K Q^T     32 x 32 x 16, the queries in registers: a lane gets 16 of 32 keys for its own column, the lane 32 further on the others
+//   O^T += V^T P^T  32 x 32 x 16: the weights as they lie are the second operand, the first comes out of LDS with transposing reads
+// A wave's stage: the softmax of the stage's scores in the vector ALU, then pairs of (one step of O^T, one step of the NEXT stage's S^T), their LDS operands asked
+// for four pairs ahead and the second half of the exponentials computed beside the first pairs.
+// The weights are rounded to the storage type for the second product, as the matrix units take them; the sum takes them rounded too.
+// Blocks come longest first; where the kv heads are a multiple of 8 the blocks of a head go to one XCD, whose L2 then fetches its rows once.
+// =================================================================================================
+typedef _Float16 f16x2 __attribute__( ( ext_vector_type( 2 ) ) );
+typedef __bf16 b16x2 __attribute__( ( ext_vector_type( 2 ) ) );
+
+// sum + the two weights of a packed pair
+template<typename E>
+__device__ __forceinline__ float add_pair( uint32_t pair, float sum )
+{
+  if constexpr ( std::is_same_v<E, __half> ) {
+    return __builtin_amdgcn_fdot2( __builtin_bit_cast( f16x2, pair ), f16x2 { (_Float16)1.0f, (_Float16)1.0f }, sum, false );
+  } else {
+    return __builtin_amdgcn_fdot2_f32_bf16( __builtin_bit_cast( b16x2, pair ), b16x2 { (__bf16)1.0f, (__bf16)1.0f }, sum, false );
+  }
+}
+
+template<typename E, int CH>
+__device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restrict__ out, const Call& a )
+{
+  constexpr uint32_t RPI = 64 / CH, IPG = 16 / RPI;          // rows of a load, loads for the wave's 16 rows
+  constexpr int SK = CH / 2, I4 = CH / 4, NP = 4 * I4;       // steps of 16 dims of the scores; blocks of 32 dims; pairs of steps of a stage
+  using X8 = typename Mfma<E>::x8;
+  __shared__ uint4 s_k0[64 * CH], s_k1[64 * CH], s_v0[64 * CH], s_v1[64 * CH]; // named apart: the loop below says at compile time which one it works on
+
+  const uint32_t wave = __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 ), lane = threadIdx.x & 63, r = lane & 31, g2 = lane >> 5;
+  uint32_t number, h;
+  if ( a.n_kv_heads % 8 == 0 ) {
+    const uint32_t slot = blockIdx.x >> 3, groups = a.n_kv_heads / 8;
+    number = slot / groups;
+    h = slot % groups * 8 + ( blockIdx.x & 7 );
+  } else {
+    number = blockIdx.x / a.n_kv_heads;
+    h = blockIdx.x % a.n_kv_heads;
+  }
+  Block b;
+  if ( !block_of<false, 128>( a, number, h, blockIdx.y, &b ) ) {
+    return;
+  }
+  const uint32_t n_heads = a.n_kv_heads * a.gqa, n_cols = b.tokens * a.gqa;
+  const uint32_t k_begin = b.split * a.chunk, k_most = k_begin + a.chunk;
+  auto end_of = [&]( uint32_t token ) { return min( visible( a, b, token ), k_most ); }; // keys a token attends of this split: [k_begin, end)
+  const uint32_t wg_end = __builtin_amdgcn_readfirstlane( end_of( ( min( n_cols, b.col0 + 128 ) - 1 ) / a.gqa ) );
+  if ( wg_end <= k_begin ) {
+    return;
+  }
+  const uint32_t first_col = b.col0 + 32 * wave;
+  const bool wave_ok = first_col < n_cols; // a wave without columns still fetches its share of every stage
+  const uint32_t t_end = __builtin_amdgcn_readfirstlane( wave_ok ? end_of( ( min( n_cols, first_col + 32 ) - 1 ) / a.gqa ) : 0 ); // of some column of the wave
+  const uint32_t t_all = __builtin_amdgcn_readfirstlane( wave_ok ? end_of( first_col / a.gqa ) : 0 );                               // of every column
+  const uint32_t col = first_col + r;
+  const bool ok = col < n_cols;
+  const uint32_t token = ok ? col / a.gqa : 0, head = h * a.gqa + ( ok ? col % a.gqa : 0 );
+  const uint32_t my_end = ok ? end_of( token ) : 0;
+  const uint64_t place = (uint64_t)( b.row0 + token ) * n_heads + head;
+
+  X8 qb[SK];
+#pragma unroll
+  for ( int s = 0; s < SK; s++ ) {
+    const uint32_t d = 8 * ( 2 * s + g2 );
+    qb[s] = ok && d < a.size ? *reinterpret_cast<const X8*>( q + place * a.size + d ) : X8 { 0, 0, 0, 0, 0, 0, 0, 0 };
+  }
+
+  mfma_f32x16 acc[I4]; // element v of acc[i]: dim 32 i + 8 (v / 4) + 4 g2 + v % 4 of the lane's column
+#pragma unroll
+  for ( int i = 0; i < I4; i++ ) {
+#pragma unroll
+    for ( int v = 0; v < 16; v++ ) {
+      acc[i][v] = 0.0f;
+    }
+  }
+  float m = -INFINITY, l = 0.0f; // m: within LAZY of the column's maximum; l: this lane's share
+
+  // a lane's place in the rows of a load; chunks behind the head far outside every descriptor
+  const uint32_t ld_row = lane / CH, ld_slot = lane % CH, chunks = a.size / 8;
+  const uint32_t k_off = h * a.size * 2, v_off = ( a.n_kv_heads + h ) * a.size * 2;
+  auto k_swizzle = []( uint32_t row ) { return CH == 16 ? row & 15 : ( row >> 1 ) & 7; };
+  auto v_swizzle = []( uint32_t row ) { return CH == 16 ? 4 * ( row & 3 ) : 4 * ( ( row >> 1 ) & 1 ); };
+  uint32_t k_at[IPG], v_at[IPG];
+#pragma unroll
+  for ( uint32_t t = 0; t < IPG; t++ ) {
+    const uint32_t row = RPI * t + ld_row, kc = ld_slot ^ k_swizzle( row ), vc = ld_slot ^ v_swizzle( row );
+    k_at[t] = kc < chunks ? row * a.pages.row_bytes + k_off + 16 * kc : 0x80000000u;
+    v_at[t] = vc < chunks ? row * a.pages.row_bytes + v_off + 16 * vc : 0x80000000u;
+  }
+  // page numbers by scalar loads, a stage before they are needed
+  typedef const uint32_t __attribute__( ( address_space( 4 ) ) ) * scalar_ptr;
+  const scalar_ptr table = (scalar_ptr)( reinterpret_cast<uintptr_t>( a.pages.table + (uint64_t)b.seq * a.pages.table_stride ) );
+  auto look_up = [&]( uint32_t stage ) __attribute__( ( always_inline ) ) { return table[min( k_begin + 64 * stage + 16 * wave, wg_end - 1 ) >> a.pages.shift]; };
+  auto describe = [&]( uint32_t stage, uint32_t id ) __attribute__( ( always_inline ) ) {
+    const uint32_t key = k_begin + 64 * stage + 16 * wave;
+    const char* base = a.pages.pool + min( id, a.pages.last ) * a.pages.stride + (uint64_t)( key & ( ( 1u << a.pages.shift ) - 1 ) ) * a.pages.row_bytes;
+    const uint32_t rows = key < wg_end ? min( wg_end - key, 16u ) : 0u;
+    return __builtin_amdgcn_make_buffer_rsrc( const_cast<char*>( base ), 0, (int)( rows * a.pages.row_bytes ), 0x00020000 );
+  };
+  auto fetch = [&]( __amdgpu_buffer_rsrc_t rsrc, uint4* tile, const uint32_t( &at )[IPG] ) __attribute__( ( always_inline ) ) {
+#pragma unroll
+    for ( uint32_t t = 0; t < IPG; t++ ) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds( rsrc, (lds_ptr)( tile + ( 16 * wave + RPI * t ) * CH ), 16, at[t], 0, 0, 0 );
+    }
+  };
+
+  // transposing reads of V: lane 4 e + p of 16 points at key slot e of its half-wave, dims 16 grp + 4 p .. + 3 of dim block 0
+  const uint32_t tr_e = ( lane & 15 ) >> 2, tr_p = lane & 3, tr_grp = ( lane >> 4 ) & 1;
+  const uint32_t v_lane = ( 4 * g2 + tr_e ) * CH * 16 + ( ( ( 2 * tr_grp + ( tr_p >> 1 ) ) ^ v_swizzle( 4 * g2 + tr_e ) ) * 16 ) + ( tr_p & 1 ) * 8;
+
+  X8 ka[4];
+  auto read_k = [&]( const uint4* kt, int n ) __attribute__( ( always_inline ) ) {
+    const uint32_t row = 32 * ( n / SK ) + r;
+    ka[n & 3] = __builtin_bit_cast( X8, kt[row * CH + ( ( 2 * ( n % SK ) + g2 ) ^ k_swizzle( r ) )] );
+  };
+  auto score_step = [&]( mfma_f32x16( &st )[2], int n ) __attribute__( ( always_inline ) ) {
+    if ( n % SK == 0 ) {
+      const mfma_f32x16 zero = { 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0 };
+      st[n / SK] = Mfma<E>::k16( ka[n & 3], qb[n % SK], zero );
+    } else {
+      st[n / SK] = Mfma<E>::k16( ka[n & 3], qb[n % SK], st[n / SK] );
+    }
+  };
+  v4s va[4][2];
+  auto read_v = [&]( const uint4* vt, int n ) __attribute__( ( always_inline ) ) {
+#pragma unroll
+    for ( int half = 0; half < 2; half++ ) {
+      va[n & 3][half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16( (lds_v4s)( (lds_char*)vt + ( v_lane ^ ( 64 * ( n % I4 ) ) ) + ( 16 * ( n / I4 ) + 8 * half ) * CH * 16 ) );
+    }
+  };
+
+  // Behind the barrier of stage i every wave is done with K of stage i (whose scores were made in stage i - 1) and with V of stage i - 1, so K of stage i + 2
+  // and V of stage i + 1 are asked for into their places; the barrier of stage i + 1 waits for them.
+  const uint32_t n_stages = ( wg_end - k_begin + 63 ) / 64, my_stages = t_end > k_begin ? ( t_end - k_begin + 63 ) / 64 : 0;
+  __amdgpu_buffer_rsrc_t next = describe( 0, look_up( 0 ) );
+  fetch( next, s_k0, k_at );
+  fetch( next, s_v0, v_at );
+  next = describe( 1, look_up( 1 ) ); // of stage i + 1
+  fetch( next, s_k1, k_at );
+  uint32_t id = look_up( 2 ); // of stage i + 2
+  __builtin_amdgcn_s_waitcnt( 0x0F70 ); // vmcnt(0)
+  __syncthreads();
+  mfma_f32x16 st_a[2], st_b[2]; // scores of even and of odd stages
+  if ( my_stages > 0 ) {
+#pragma unroll
+    for ( int n = 0; n < 4; n++ ) {
+      read_k( s_k0, n );
+    }
+#pragma unroll
+    for ( int n = 0; n < NP; n++ ) {
+      score_step( st_a, n );
+      if ( n + 4 < NP ) {
+        read_k( s_k0, n + 4 );
+      }
+    }
+  }
+
+  auto stage = [&]( uint32_t i, uint4* k_cur, uint4* v_cur, uint4* k_nxt, uint4* v_nxt, mfma_f32x16( &st )[2], mfma_f32x16( &st_nxt )[2] ) __attribute__( ( always_inline ) ) {
+    const uint32_t t0 = k_begin + 64 * i;
+    __builtin_amdgcn_s_waitcnt( 0x0F70 ); // vmcnt(0): what this wave asked for has landed, behind the barrier what all did
+    __syncthreads();
+    if ( i + 1 < n_stages ) {
+      fetch( next, v_nxt, v_at );
+    }
+    if ( i + 2 < n_stages ) {
+      next = describe( i + 2, id );
+      fetch( next, k_cur, k_at );
+      id = look_up( i + 3 );
+    }
+    if ( i >= my_stages ) {
+      return; // the whole wave
+    }
+#pragma unroll
+    for ( int n = 0; n < 4; n++ ) { // the softmax gives them the time to arrive
+      read_v( v_cur, n );
+      read_k( k_nxt, n );
+    }
+    __builtin_amdgcn_sched_barrier( 0 );
+    if ( __builtin_amdgcn_readfirstlane( t0 + 64 > t_all ) ) { // keys that some column does not see
+      asm volatile( "" ::: "memory" ); // keeps this a branch: the selects are only paid for here
+#pragma unroll
+      for ( int sub = 0; sub < 2; sub++ ) {
+#pragma unroll
+        for ( int v = 0; v < 16; v++ ) {
+          st[sub][v] = t0 + 32 * sub + 8 * ( v / 4 ) + 4 * g2 + ( v % 4 ) < my_end ? st[sub][v] : -INFINITY;
+        }
+      }
+    }
+    float m4[4]; // independent chains
+#pragma unroll
+    for ( int c = 0; c < 4; c++ ) {
+      m4[c] = st[c >> 1][8 * ( c & 1 )];
+#pragma unroll
+      for ( int e = 1; e < 8; e++ ) {
+        m4[c] = fmaxf( m4[c], st[c >> 1][8 * ( c & 1 ) + e] );
+      }
+    }
+    const float mx = half_wave_max( fmaxf( fmaxf( m4[0], m4[1] ), fmaxf( m4[2], m4[3] ) ) ) * a.scale_log2e;
+    if ( __builtin_amdgcn_ballot_w64( mx > m + LAZY ) != 0 ) {
+      const float m_new = fmaxf( m, mx ), alpha = m_new == -INFINITY ? 1.0f : fast_exp2( m - m_new );
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for ( int i4 = 0; i4 < I4; i4++ ) {
+#pragma unroll
+        for ( int v = 0; v < 16; v++ ) {
+          acc[i4][v] *= alpha;
+        }
+      }
+    }
+    const float ms = m == -INFINITY ? 0.0f : m;
+    // weights of keys 16 kk .. 16 kk + 15, packed as the second operand of their steps
+    typedef uint32_t u32x4 __attribute__( ( ext_vector_type( 4 ) ) );
+    u32x4 pk[4];
+    float sum[2] = { 0.0f, 0.0f };
+    auto weights = [&]( int kk, int e0 ) __attribute__( ( always_inline ) ) {
+      float p[2];
+#pragma unroll
+      for ( int e = 0; e < 2; e++ ) {
+        p[e] = fast_exp2( st[kk >> 1][8 * ( kk & 1 ) + e0 + e] * a.scale_log2e - ms );
+      }
+      const uint32_t pair = rounded_pair<E>( p[0], p[1] );
+      sum[( e0 >> 1 ) & 1] = add_pair<E>( pair, sum[( e0 >> 1 ) & 1] );
+      pk[kk][e0 >> 1] = pair;
+    };
+#pragma unroll
+    for ( int kk = 0; kk < 2; kk++ ) {
+#pragma unroll
+      for ( int e0 = 0; e0 < 8; e0 += 2 ) {
+        weights( kk, e0 );
+      }
+    }
+    __builtin_amdgcn_sched_barrier( 0 );
+#pragma unroll
+    for ( int n = 0; n < NP; n++ ) {
+      const int kk = n / I4, i4 = n % I4;
+      const v4s lo = va[n & 3][0], hi = va[n & 3][1];
+      acc[i4] = Mfma<E>::k16( __builtin_bit_cast( X8, ( v8s { lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3] } ) ), __builtin_bit_cast( X8, pk[kk] ), acc[i4] );
+      score_step( st_nxt, n ); // (behind the wave's last stage nothing uses them)
+      if ( n + 4 < NP ) {
+        read_v( v_cur, n + 4 );
+        read_k( k_nxt, n + 4 );
+      }
+      if ( n < NP / 2 ) { // vector ALU work beside the matrix units
+#pragma unroll
+        for ( int e0 = 8 / I4 * i4; e0 < 8 / I4 * ( i4 + 1 ); e0 += 2 ) {
+          weights( 2 + kk, e0 );
+        }
+      }
+      __builtin_amdgcn_sched_barrier( 0 );
+    }
+    l += sum[0] + sum[1];
+  };
+  for ( uint32_t i = 0; i < n_stages; i += 2 ) {
+    stage( i, s_k0, s_v0, s_k1, s_v1, st_a, st_b );
+    if ( i + 1 < n_stages ) {
+      stage( i + 1, s_k1, s_v1, s_k0, s_v0, st_b, st_a );
+    }
+  }
+
+  l += __shfl_xor( l, 32, WAVE );
+  float probe = l;
+#pragma unroll
+  for ( int i = 0; i < I4; i++ ) {
+#pragma unroll
+    for ( int v = 0; v < 16; v++ ) {
+      probe += 0.0f * acc[i][v];
+    }
+  }
+  const bool mine = ok && k_begin < my_end;
+  const uint64_t bad = __builtin_amdgcn_ballot_w64( mine && probe != probe );
+  uint32_t again = (uint32_t)bad | (uint32_t)( bad >> 32 ); // columns with a NaN: once more key by key
+  if ( mine && !( again >> r & 1 ) ) {
+    if ( a.splits > 1 ) {
+      const uint64_t slot = place * a.splits + b.split;
+#pragma unroll
+      for ( int i = 0; i < I4; i++ ) {
+#pragma unroll
+        for ( int v = 0; v < 16; v += 4 ) {
+          const uint32_t d = 32 * i + 2 * v + 4 * g2;
+          if ( d < a.size ) {
+            *reinterpret_cast<float4*>( a.part_out + slot * a.size + d ) = make_float4( acc[i][v], acc[i][v + 1], acc[i][v + 2], acc[i][v + 3] );
+          }
+        }
+      }
+      if ( g2 == 0 ) {
+        a.part_ml[slot * 2] = m;
+        a.part_ml[slot * 2 + 1] = l;
+      }
+    } else {
+      const float inv = 1.0f / l;
+#pragma unroll
+      for ( int i = 0; i < I4; i++ ) {
+#pragma unroll
+        for ( int v = 0; v < 16; v += 4 ) {
+          const uint32_t d = 32 * i + 2 * v + 4 * g2;
+          if ( d < a.size ) {
+            *reinterpret_cast<uint2*>( out + place * a.size + d )
+              = make_uint2( rounded_pair<E>( acc[i][v] * inv, acc[i][v + 1] * inv ), rounded_pair<E>( acc[i][v + 2] * inv, acc[i][v + 3] * inv ) );
+          }
+        }
+      }
+    }
+  }
+  while ( again != 0 ) {
+    const uint32_t cl = first_col + (uint32_t)__builtin_ctz( again );
+    again &= again - 1;
+    walk_column<E>( q, out, a, b, cl, k_begin, end_of( cl / a.gqa ) );
+  }
+}
+
+template<typename E, int CH>
+__global__ __launch_bounds__( 256, 2 ) void attn_pages_packed_kernel( const E* __restrict__ q, E* __restrict__ out, Call a )
+{
+  packed_run<E, CH>( q, out, a );
+}
+
+// =================================================================================================
+// splits of a row added up: NW waves of a work-group take a (query row, head), every NW-th split each, eight of them asked for at once
+// =================================================================================================
+template<typename T, bool DECODE, int NW>
+__global__ __launch_bounds__( 256 ) void pages_merge_kernel( T* __restrict__ out, Call a, uint32_t rows )
+{
+  constexpr int PER = 4 / NW; // (row, head)s of a work-group
+  __shared__ float s_part[4][256], s_l[4];
+  const uint32_t lane = threadIdx.x & 63, n_heads = a.n_kv_heads * a.gqa, wave = __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 ), turn = wave % NW;
+  const uint64_t place = (uint64_t)blockIdx.x * PER + wave / NW;
+  const uint32_t row = (uint32_t)( place / n_heads );
+  uint32_t keys = 0;
+  if ( row < rows ) {
+    if constexpr ( DECODE ) {
+      keys = min( a.lengths[row], a.max_keys );
+    } else {
+      const uint32_t seq = packed_sequence( a.seqs, row );
+      if ( seq < a.seqs.batch && row - a.seqs.begin( seq ) < a.seqs.count( seq ) ) {
+        const uint32_t start = a.seqs.start ? min( a.seqs.start[seq], 0x7fffffffu ) : 0u;
+        keys = min( start + ( row - a.seqs.begin( seq ) ) + 1, a.max_keys );
+      }
+    }
+  }
+  const uint32_t n = ( keys + a.chunk - 1 ) / a.chunk; // at most a.splits, as max_keys is at most splits * chunk
   const float* ml = a.part_ml + place * a.splits * 2;
   const float* part = a.part_out + place * a.splits * a.size;
   float mm = -INFINITY;
@@ -392,27 +1063,56 @@ __global__ __launch_bounds__( 256 ) void pages_merge_kernel( T* __restrict__ out
   mm = wave_max( mm );
   const float mm_safe = mm == -INFINITY ? 0.0f : mm;
   float l = 0.0f, acc[4] = { 0, 0, 0, 0 };
-  for ( uint32_t s0 = 0; s0 < n; s0 += 64 ) {
-    float w = 0.0f, ls = 0.0f;
-    if ( s0 + lane < n ) {
-      w = fast_exp2( ml[2 * ( s0 + lane )] - mm_safe );
-      ls = ml[2 * ( s0 + lane ) + 1];
-    }
-    l += wave_sum( w * ls );
-    const uint32_t k = min( 64u, n - s0 );
-    for ( uint32_t s = 0; s < k; s++ ) {
-      const float ws = __shfl( w, (int)s, WAVE );
+  for ( uint32_t s0 = 0; s0 < n; s0 += 64 * NW ) { // lane <-> split s0 + NW lane + turn
+    const uint32_t mine = s0 + NW * lane + turn;
+    const float w = mine < n ? fast_exp2( ml[2 * mine] - mm_safe ) : 0.0f;
+    l += wave_sum( mine < n ? w * ml[2 * mine + 1] : 0.0f );
+    for ( uint32_t k0 = 0; k0 < 64 && s0 + NW * k0 + turn < n; k0 += 8 ) {
+      float v[8][4];
 #pragma unroll
-      for ( int u = 0; u < 4; u++ ) {
-        const uint32_t d = 64 * u + lane;
-        if ( d < a.size ) {
-          acc[u] = __builtin_fmaf( part[(uint64_t)( s0 + s ) * a.size + d], ws, acc[u] );
+      for ( uint32_t k = 0; k < 8; k++ ) {
+        const uint32_t split = min( s0 + NW * ( k0 + k ) + turn, n - 1 ); // past the end: the last one, whose weight there is 0 (its values may be infinite)
+#pragma unroll
+        for ( uint32_t u = 0; u < 4; u++ ) {
+          v[k][u] = 64 * u + lane < a.size ? part[(uint64_t)split * a.size + 64 * u + lane] : 0.0f;
+        }
+      }
+#pragma unroll
+      for ( uint32_t k = 0; k < 8; k++ ) {
+        const float wk = lane_value( w, (int)( k0 + k ) );
+        const bool there = s0 + NW * ( k0 + k ) + turn < n;
+#pragma unroll
+        for ( uint32_t u = 0; u < 4; u++ ) {
+          acc[u] = there ? __builtin_fmaf( v[k][u], wk, acc[u] ) : acc[u];
         }
       }
     }
   }
+  if constexpr ( NW > 1 ) {
 #pragma unroll
-  for ( int u = 0; u < 4; u++ ) {
+    for ( uint32_t u = 0; u < 4; u++ ) {
+      s_part[wave][64 * u + lane] = acc[u];
+    }
+    if ( lane == 0 ) {
+      s_l[wave] = l;
+    }
+    __syncthreads();
+    if ( turn != 0 ) {
+      return;
+    }
+    for ( uint32_t w = 1; w < NW; w++ ) {
+      l += s_l[wave + w];
+#pragma unroll
+      for ( uint32_t u = 0; u < 4; u++ ) {
+        acc[u] += s_part[wave + w][64 * u + lane];
+      }
+    }
+  }
+  if ( n == 0 ) {
+    return; // a row that attends nothing is left as it is
+  }
+#pragma unroll
+  for ( uint32_t u = 0; u < 4; u++ ) {
     const uint32_t d = 64 * u + lane;
     if ( d < a.size ) {
       out[place * a.size + d] = from_f32<T>( acc[u] / l );
@@ -427,23 +1127,73 @@ struct Plan
 {
   uint32_t blocks, splits, chunk; // blocks: grid x
   uint32_t n_blocks;
+  uint32_t waves; // of a work-group of the 16-bit kernel; 0: the fp32 tile kernel
   uint64_t bytes;
 };
 
-// Keys of a split: whole numbers of 64.  As many splits as bring the launch to four work-groups a CU, of at least 256 keys.
-Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, const gh_shape* s )
+// The 16-bit kernels take heads made of 16-byte chunks, runs of 16 keys in one page, and everything aligned to 16 bytes.
+bool takes16( const gh_shape* s, gh_dtype dt )
+{
+  return dt != GH_F32 && s->head_size % 8 == 0 && s->head_size <= 128;
+}
+
+constexpr uint64_t MOST_PARTS = 65536; // of (query row, head, split) that leave partial results
+
+// How a call is cut.  Splits are whole numbers of 64 keys.
+Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, const gh_shape* s, bool tiles16 )
 {
   Plan p {};
-  const uint32_t cols = decode ? 16 : 64;
+  const uint32_t cols = decode ? 16 : tiles16 ? 128 : 64;
   p.n_blocks = decode ? ( s->gqa_size + cols - 1 ) / cols : 0;
   const uint64_t blocks = decode ? batch * p.n_blocks : std::min<uint64_t>( ( rows * s->gqa_size + cols - 1 ) / cols + batch, rows * s->gqa_size );
   p.blocks = (uint32_t)blocks;
-  const uint64_t groups = blocks * s->n_kv_heads;
-  uint64_t splits = std::max<uint64_t>( 1, std::min<uint64_t>( 4ull * (uint64_t)cu_count() / groups, ( max_keys + 255 ) / 256 ) );
+  if ( decode && tiles16 ) {
+    // Microseconds as measured on MI355X.  A stage of 32 keys takes a wave on its own 0.75, the four waves of a work-group 1.5, and 2.4 where the waves that fit
+    // (four a CU at 128 elements) share the memory's rate; a round of work-groups takes 2 to begin and end; a split adds a launch (4) and 8 bytes an element
+    // that go out and come back at 3 TB/s.  Where lengths differ the launch ends on the longest runs: a tenth of a wave's stages.
+    // Measured, GQA heads (8 of 8 queries) in f16, us: 1 context of 301 keys, 4 waves 7.0, splits of 64 8.8 | 1 x 4096, 4 waves unsplit 39, splits of 64 10.8 |
+    // 16 x 500, 4 waves 9.8, one wave 15.1 | 64 x 4096, splits of 2048 167, of 512 185, of 64 261 | 256 x 1000, one wave 162, 4 waves 177
+    // 32 heads of one query: 8 x 2000, 4 waves 42, one wave 48 | 3 x 30000, splits of 1024 233, of 128 248, 4 waves unsplit 269
+    const uint64_t streams = batch * p.n_blocks * s->n_kv_heads;
+    const double slots = 4.0 * cu_count() * ( s->head_size <= 64 ? 2 : 1 );
+    double best = 0;
+    for ( uint32_t waves = 1; waves <= 4; waves += 3 ) {
+      for ( uint32_t chunk = 64; chunk != 0; chunk = chunk >= max_keys ? 0 : 2 * chunk ) {
+        const uint64_t splits = ( max_keys + chunk - 1 ) / chunk;
+        if ( splits > 65535 || ( splits > 1 && rows * s->n_heads * splits > MOST_PARTS ) ) {
+          continue;
+        }
+        const double stages = (double)( ( std::min( chunk, max_keys ) + 32 * waves - 1 ) / ( 32 * waves ) ), load = (double)( streams * splits * waves ) / slots;
+        const double alone = waves == 1 ? 0.75 : 1.5, full = std::max( alone, 2.4 * std::min( 1.0, load ) );
+        double us = stages * std::max( alone, 2.4 * load ) + 0.1 * stages * full + 2.0 * std::max( 1.0, load );
+        if ( splits > 1 ) {
+          us += 4.0 + (double)( rows * s->n_heads * splits ) * s->head_size * 8 / 3e6;
+        }
+        if ( p.waves == 0 || us < best ) {
+          best = us;
+          p.waves = waves;
+          p.chunk = chunk;
+          p.splits = (uint32_t)splits;
+        }
+      }
+    }
+    p.bytes = p.splits == 1 ? 0 : rows * s->n_heads * p.splits * ( s->head_size + 2 ) * sizeof( float );
+    return p;
+  }
+  // as many splits as bring the launch to four work-groups a CU (two of the 16-bit kernel), of at least 256 keys
+  const uint64_t groups = blocks * s->n_kv_heads, wanted = ( tiles16 ? 2ull : 4ull ) * (uint64_t)cu_count();
+  const uint64_t splits = std::max<uint64_t>( 1, std::min( { wanted / groups, (uint64_t)( max_keys + 255 ) / 256, MOST_PARTS / ( rows * s->n_heads ) } ) );
+  p.waves = tiles16 ? 4 : 0;
   p.chunk = (uint32_t)( ( ( max_keys + splits - 1 ) / splits + 63 ) / 64 * 64 );
   p.splits = ( max_keys + p.chunk - 1 ) / p.chunk;
   p.bytes = p.splits == 1 ? 0 : rows * s->n_heads * p.splits * ( s->head_size + 2 ) * sizeof( float );
   return p;
+}
+
+// Bytes that every plan of at most so many rows and keys fits into.
+uint64_t most_bytes( uint64_t rows, uint32_t max_keys, const gh_shape* s )
+{
+  return max_keys <= 64 ? 0 : std::min<uint64_t>( rows * s->n_heads * ( ( (uint64_t)max_keys + 63 ) / 64 ), MOST_PARTS ) * ( s->head_size + 2 ) * sizeof( float );
 }
 
 bool shape_ok( const gh_shape* s )
@@ -467,13 +1217,67 @@ void launch_f32( const Plan& p, const Call& a, const void* q, void* out, hipStre
   }
 }
 
+template<typename E>
+void launch_decode16( const Plan& p, const Call& a, const void* q, void* out, hipStream_t st )
+{
+  const E* tq = static_cast<const E*>( q );
+  E* to = static_cast<E*>( out );
+  auto go = [&]( auto chunks, auto waves, auto heads ) {
+    constexpr int CH = decltype( chunks )::value, W = decltype( waves )::value, HW = decltype( heads )::value;
+    attn_pages_decode_kernel<E, CH, W, HW><<<dim3( p.blocks * ( a.n_kv_heads / HW ), p.splits ), 64 * W * HW, 0, st>>>( tq, to, a );
+  };
+  const std::integral_constant<int, 1> one {};
+  const std::integral_constant<int, 2> two {};
+  const std::integral_constant<int, 4> four {};
+  auto sizes = [&]( auto chunks ) {
+    if ( p.waves > 1 ) {
+      go( chunks, four, one );
+    } else if ( a.n_kv_heads % 2 == 0 ) {
+      go( chunks, one, two );
+    } else {
+      go( chunks, one, one );
+    }
+  };
+  if ( a.size <= 64 ) {
+    sizes( std::integral_constant<int, 8> {} );
+  } else {
+    sizes( std::integral_constant<int, 16> {} );
+  }
+}
+
+template<typename E>
+void launch_packed16( const Plan& p, const Call& a, const void* q, void* out, hipStream_t st )
+{
+  const dim3 grid( p.blocks * a.n_kv_heads, p.splits );
+  if ( a.size <= 64 ) {
+    attn_pages_packed_kernel<E, 8><<<grid, 256, 0, st>>>( static_cast<const E*>( q ), static_cast<E*>( out ), a );
+  } else {
+    attn_pages_packed_kernel<E, 16><<<grid, 256, 0, st>>>( static_cast<const E*>( q ), static_cast<E*>( out ), a );
+  }
+}
+
 template<typename T, bool DECODE>
 int launch( const Plan& p, const Call& a, const void* q, void* out, uint64_t rows, hipStream_t st )
 {
-  launch_f32<T, DECODE>( p, a, q, out, st );
+  if constexpr ( sizeof( T ) == 2 ) {
+    if ( p.waves != 0 && DECODE ) {
+      launch_decode16<T>( p, a, q, out, st );
+    } else if ( p.waves != 0 ) {
+      launch_packed16<T>( p, a, q, out, st );
+    } else {
+      launch_f32<T, DECODE>( p, a, q, out, st );
+    }
+  } else {
+    launch_f32<T, DECODE>( p, a, q, out, st );
+  }
   GH_LAUNCH_CHECK();
   if ( p.splits > 1 ) {
-    pages_merge_kernel<T, DECODE><<<(unsigned)( ( rows * a.n_kv_heads * a.gqa + 3 ) / 4 ), 256, 0, st>>>( static_cast<T*>( out ), a, (uint32_t)rows );
+    const uint64_t places = rows * a.n_kv_heads * a.gqa;
+    if ( places < 16ull * (uint64_t)cu_count() ) {
+      pages_merge_kernel<T, DECODE, 4><<<(unsigned)places, 256, 0, st>>>( static_cast<T*>( out ), a, (uint32_t)rows );
+    } else {
+      pages_merge_kernel<T, DECODE, 1><<<(unsigned)( ( places + 3 ) / 4 ), 256, 0, st>>>( static_cast<T*>( out ), a, (uint32_t)rows );
+    }
     GH_LAUNCH_CHECK();
   }
   return GH_OK;
@@ -503,7 +1307,8 @@ int attn_pages( const char* op, const void* q, const gh_pages* pages, const uint
   if ( empty ) {
     return GH_OK;
   }
-  const Plan p = plan_call( DECODE, batch, rows, max_keys, s );
+  const uint64_t places = reinterpret_cast<uintptr_t>( pages->pool ) | pages->page_stride | reinterpret_cast<uintptr_t>( q ) | reinterpret_cast<uintptr_t>( xb );
+  const Plan p = plan_call( DECODE, batch, rows, max_keys, s, takes16( s, dt ) && places % 16 == 0 && pages->page_tokens >= 16 );
   GH_REQUIRE( p.bytes == 0 || ( workspace != nullptr && reinterpret_cast<uintptr_t>( workspace ) % 16 == 0 ), "%s: a 16-byte aligned workspace is needed", op );
   if ( p.bytes > workspace_bytes ) {
     return fail( GH_ERR_WORKSPACE, "%s: workspace of %llu bytes, %llu are needed", op, (unsigned long long)workspace_bytes, (unsigned long long)p.bytes );
@@ -537,7 +1342,7 @@ extern "C" {
 
 uint64_t gh_attn_decode_paged_workspace( uint64_t batch, uint32_t max_length, const gh_shape* shape, gh_dtype dt )
 {
-  return !shape_ok( shape ) || batch == 0 || max_length == 0 ? 0 : plan_call( true, batch, batch, max_length, shape ).bytes;
+  return !shape_ok( shape ) || batch == 0 || batch > 1u << 24 ? 0 : most_bytes( batch, max_length, shape );
 }
 
 int gh_attn_decode_paged( const void* q, const gh_pages* pages, const uint32_t* lengths_dev, void* xb, uint64_t batch, uint32_t max_length, const gh_shape* shape,
@@ -548,7 +1353,7 @@ int gh_attn_decode_paged( const void* q, const gh_pages* pages, const uint32_t* 
 
 uint64_t gh_attn_packed_workspace( uint64_t batch, uint64_t n_tokens, uint32_t max_keys, const gh_shape* shape, gh_dtype dt )
 {
-  return !shape_ok( shape ) || batch == 0 || n_tokens == 0 || max_keys == 0 ? 0 : plan_call( false, batch, n_tokens, max_keys, shape ).bytes;
+  return !shape_ok( shape ) || batch == 0 || n_tokens > 1u << 24 ? 0 : most_bytes( n_tokens, max_keys, shape );
 }
 
 int gh_attn_packed( const void* q, const gh_pages* pages, const uint32_t* first_dev, const uint32_t* start_pos_dev, void* xb, uint64_t batch, uint64_t n_tokens,
