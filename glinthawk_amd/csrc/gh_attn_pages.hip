@@ -55,14 +55,16 @@ __device__ __forceinline__ bool block_of( const Call& a, uint32_t number, uint32
     b->start = length - 1;
     return true;
   } else {
-    uint32_t block;
-    if ( !packed_block( a.seqs, a.gqa, COLS, number, &b->seq, &block ) ) {
+    uint32_t seq, block;
+    if ( !packed_block( a.seqs, a.gqa, COLS, number, &seq, &block ) ) {
       return false;
     }
-    b->col0 = block * COLS;
-    b->row0 = a.seqs.begin( b->seq );
-    b->tokens = a.seqs.count( b->seq );
-    b->start = a.seqs.start ? min( a.seqs.start[b->seq], 0x7fffffffu ) : 0u;
+    // (said to be the same in every lane: what descriptors and branches are made of stays in scalar registers)
+    b->seq = __builtin_amdgcn_readfirstlane( seq );
+    b->col0 = __builtin_amdgcn_readfirstlane( block ) * COLS;
+    b->row0 = __builtin_amdgcn_readfirstlane( a.seqs.begin( b->seq ) );
+    b->tokens = __builtin_amdgcn_readfirstlane( a.seqs.count( b->seq ) );
+    b->start = __builtin_amdgcn_readfirstlane( a.seqs.start ? min( a.seqs.start[b->seq], 0x7fffffffu ) : 0u );
     return true;
   }
 }
@@ -383,7 +385,7 @@ typedef __attribute__( ( address_space( 3 ) ) ) v4s* lds_v4s;
 constexpr float LAZY = 8.0f; // the reference point of the exponentials stays until a maximum is 2^LAZY above it: weights up to 256, fewer rescalings
 
 // maximum over the lanes that share a column, 16 lanes apart, without a trip through LDS
-__device__ __forceinline__ float column_max( float v )
+[[maybe_unused]] __device__ __forceinline__ float column_max( float v )
 {
   v = half_wave_max( v );
   const unsigned bits = __builtin_bit_cast( unsigned, v );

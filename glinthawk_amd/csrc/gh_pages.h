@@ -118,8 +118,8 @@ __device__ __forceinline__ bool packed_block( const Packed& s, uint32_t gqa, uin
     if ( rank < n ) {
       // the lane whose set bit has `rank` set bits below it
       const uint64_t hit = __builtin_amdgcn_ballot_w64( ( have >> lane & 1 ) && (uint32_t)__popcll( have & ( ( 1ull << lane ) - 1 ) ) == rank );
-      *seq = __builtin_amdgcn_readfirstlane( i0 + (uint32_t)__builtin_ctzll( hit ) );
-      *block = __builtin_amdgcn_readfirstlane( low );
+      *seq = i0 + (uint32_t)__builtin_ctzll( hit );
+      *block = low;
       return true;
     }
     rank -= n;
