@@ -4,12 +4,13 @@
 //   ln p(x) = x - m - ln S,   entropy = - sum p ln p = ln S - T / S.
 // All three are kept as a pass goes: where the maximum grows by d, S becomes e^-d S and T becomes e^-d (T - d S).
 //
-// A part of a row is held in the registers of a work-group, so that the logits are read once, all pieces asked for at the start.  The largest values come out of
-// them as whole numbers: a value's bits in the order of the values, then its index the other way round, so that no two are equal and the lower index of equal
-// values is the larger number.  Every thread knows its own largest; a wave's n-th largest of those is a number that n values at least reach, and so is the
-// largest such number of all waves.  What reaches it (mostly a few times n) goes to LDS and is ranked by counting; where that are more than fit, the numbers come
+// A part of a row is held in the registers of a work-group, so that the logits are read once, all pieces asked for at the start: bound by the bytes for many rows (and
+// nearly by the vector ALU: some 12 slots a value), by latency for few.
+// The largest values: of the threads' own largest, each wave knows the q-th; half the waves have q threads that reach the middle one of those, so with q = 2 n / waves
+// at least n values do, and of many thousand only some more.  They go to LDS as whole numbers, a value's bits in the order of the values, then its index the other way
+// round, so that no two are equal and the lower index of equal values is the larger number, and are ranked by counting; where they are more than fit, the numbers come
 // out one after the other, each the largest below the one before.
-// Rows of one part are finished by their work-group.  Longer ones, and few rows, are cut into parts whose S, T, m and sorted largest numbers a second kernel joins.
+// Rows of one part are finished by their work-group.  Longer ones are cut into parts whose S, T, m and sorted largest numbers a second kernel joins.
 #include "gh_common.h"
 
 #include <algorithm>
@@ -52,6 +53,51 @@ __device__ __forceinline__ uint64_t wave_max_u64( uint64_t v )
   return v;
 }
 
+// the k-th largest value of a wave's lanes (equal ones count each), without NaN; k at most 64
+__device__ __forceinline__ float largest_of( float v, uint32_t k )
+{
+  for ( ;; ) {
+    const float t = wave_max( v );
+    const uint32_t n = (uint32_t)__popcll( __builtin_amdgcn_ballot_w64( v == t ) );
+    if ( n >= k || t == -INFINITY ) {
+      return t;
+    }
+    k -= n;
+    v = v == t ? -INFINITY : v;
+  }
+}
+
+// 16 bytes of a row
+template<typename T>
+struct RowPiece
+{
+  static constexpr int V = 16 / sizeof( T );
+  union
+  {
+    uint4 raw;
+    T e[V];
+  };
+  // Each pass over the registers makes fp32 values of its own: kept from one to the next they would take twice the registers of the pieces.
+  __device__ __forceinline__ void forget() { asm volatile( "" : "+v"( raw.x ), "+v"( raw.y ), "+v"( raw.z ), "+v"( raw.w ) ); }
+  __device__ __forceinline__ float best() const // without NaN
+  {
+    if constexpr ( std::is_same_v<T, __half> ) { // two at a time
+      typedef _Float16 f16x2 __attribute__( ( ext_vector_type( 2 ) ) );
+      const f16x2 a = __builtin_elementwise_max( __builtin_bit_cast( f16x2, raw.x ), __builtin_bit_cast( f16x2, raw.y ) );
+      const f16x2 b = __builtin_elementwise_max( __builtin_bit_cast( f16x2, raw.z ), __builtin_bit_cast( f16x2, raw.w ) );
+      const f16x2 c = __builtin_elementwise_max( a, b );
+      return fmaxf( fmaxf( -INFINITY, (float)c.x ), (float)c.y );
+    } else {
+      float b = -INFINITY;
+#pragma unroll
+      for ( int k = 0; k < V; k++ ) {
+        b = fmaxf( b, to_f32( e[k] ) );
+      }
+      return b;
+    }
+  }
+};
+
 struct Sums
 {
   float m, s, t;
@@ -69,6 +115,13 @@ __device__ __forceinline__ Sums join( Sums a, Sums b )
   return r;
 }
 
+// S and T from sums over 2^d and 2^d d with d = x log2(e) - c: c is m log2(e) but for its rounding, which is taken out here
+__device__ __forceinline__ Sums sums_of( float max_m, float m, float c, float s, float t )
+{
+  const float off = __builtin_fmaf( m, LOG2E, -c ); // x log2(e) - c = (x - m) log2(e) + off
+  return { max_m, s * __builtin_amdgcn_exp2f( -off ), __builtin_amdgcn_exp2f( -off ) * ( __builtin_fmaf( -off, s, t ) * 0.693147180559945309417f ) };
+}
+
 __device__ __forceinline__ void finish_row( const Outputs& o, uint64_t row, Sums z, const uint32_t* tokens, uint32_t vocab, float given )
 {
   const float m = z.m == -INFINITY ? 0.0f : z.m;
@@ -83,16 +136,13 @@ __device__ __forceinline__ void finish_row( const Outputs& o, uint64_t row, Sums
 
 // grid: (parts, rows); a part: `per_part` columns, at most THREADS * PIECES * V.  One part: the row is finished here, else parts go to `sums`, `tops`.
 template<typename T, int THREADS, int PIECES>
-__global__ __launch_bounds__( THREADS ) void logprob_kernel( Outputs o, const T* __restrict__ logits, uint64_t row_stride, const uint32_t* __restrict__ tokens, uint32_t vocab,
+__global__ __launch_bounds__( THREADS, THREADS == 1024 ? ( PIECES * 16 / sizeof( T ) <= 32 ? 8 : 4 ) : 4 ) void logprob_kernel( Outputs o, const T* __restrict__ logits, uint64_t row_stride, const uint32_t* __restrict__ tokens, uint32_t vocab,
                                                             uint32_t n_top, uint32_t per_part, Sums* __restrict__ sums, uint64_t* __restrict__ tops )
 {
   constexpr int V = 16 / sizeof( T ), WAVES = THREADS / WAVE;
-  struct Piece
-  {
-    T e[V];
-  };
-  __shared__ Sums s_sums[WAVES];
-  __shared__ uint64_t s_reach[WAVES];
+  using Piece = RowPiece<T>;
+  __shared__ float2 s_sums[WAVES];
+  __shared__ float s_best[WAVES], s_reach[WAVES];
   __shared__ uint64_t s_number[CANDIDATES];
   __shared__ uint32_t s_count;
   const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
@@ -104,8 +154,8 @@ __global__ __launch_bounds__( THREADS ) void logprob_kernel( Outputs o, const T*
 #pragma unroll
   for ( int p = 0; p < PIECES; p++ ) {
     const uint32_t i = ( p * THREADS + threadIdx.x ) * V;
-    if ( i + V <= n ) {
-      __builtin_memcpy( &piece[p], x + c0 + i, 16 ); // rows may begin anywhere
+    if ( i + V <= n ) { // rows may begin anywhere
+      __builtin_memcpy( &piece[p].raw, x + c0 + i, 16 );
     } else {
 #pragma unroll
       for ( int e = 0; e < V; e++ ) {
@@ -121,58 +171,73 @@ __global__ __launch_bounds__( THREADS ) void logprob_kernel( Outputs o, const T*
     s_count = 0;
   }
 
-  Sums z { -INFINITY, 0.0f, 0.0f };
-  uint32_t best_i = 0;
+  float best = -INFINITY, piece_best[PIECES];
 #pragma unroll
   for ( int p = 0; p < PIECES; p++ ) {
-#pragma unroll
-    for ( int e = 0; e < V; e++ ) {
-      const float v = to_f32( piece[p].e[e] );
-      best_i = v > z.m ? ( p * THREADS + threadIdx.x ) * V + e : best_i; // the first of equal ones, as indices rise
-      z.m = fmaxf( z.m, v );
-    }
+    piece_best[p] = piece[p].best();
+    piece[p].forget();
+    best = fmaxf( best, piece_best[p] );
   }
-  const float m = z.m == -INFINITY ? 0.0f : z.m;
-  float s4[4] = { 0, 0, 0, 0 }, t4[4] = { 0, 0, 0, 0 };
+  const float wave_best = wave_max( best );
+  const float wave_reach = n_top == 0 ? 0.0f : largest_of( best, ( n_top + WAVES / 2 - 1 ) / ( WAVES / 2 ) );
+  if ( lane == 0 ) {
+    s_best[wave] = wave_best;
+    s_reach[wave] = wave_reach;
+  }
+  __syncthreads();
+  const float max_m = wave_max( lane < WAVES ? s_best[lane] : -INFINITY ), m = max_m == -INFINITY ? 0.0f : max_m, c = m * LOG2E;
+  float s4[4] = { 0, 0, 0, 0 }, t4[4] = { 0, 0, 0, 0 }; // in powers of 2, relative to 2^c: see `sums_of`
 #pragma unroll
   for ( int p = 0; p < PIECES; p++ ) {
 #pragma unroll
     for ( int e = 0; e < V; e++ ) {
-      const float d = to_f32( piece[p].e[e] ) - m, w = __builtin_amdgcn_exp2f( d * LOG2E );
+      const float d = __builtin_fmaf( to_f32( piece[p].e[e] ), LOG2E, -c ), w = __builtin_amdgcn_exp2f( d ); // one rounding, f16 taken as it is
       s4[e & 3] += w;
       t4[e & 3] = __builtin_fmaf( w, fmaxf( d, -1e30f ), t4[e & 3] ); // (a weight of 0 times -inf counts nothing)
     }
+    piece[p].forget();
   }
-  z.s = ( s4[0] + s4[1] ) + ( s4[2] + s4[3] );
-  z.t = ( t4[0] + t4[1] ) + ( t4[2] + t4[3] );
-  const uint64_t mine = z.m == -INFINITY ? 0 : number_of( z.m, best_i );
-#pragma unroll
-  for ( int off = 1; off < WAVE; off <<= 1 ) {
-    z = join( z, Sums { __shfl_xor( z.m, off, WAVE ), __shfl_xor( z.s, off, WAVE ), __shfl_xor( z.t, off, WAVE ) } );
-  }
-  uint64_t reach = 0;
-  if ( n_top != 0 ) {
-    uint32_t rank = 0; // lanes of the wave with a larger number (or an equal one, no value, and a lower lane)
-#pragma unroll 4
-    for ( uint32_t i = 0; i < WAVE; i++ ) {
-      const uint64_t other = (uint64_t)__builtin_amdgcn_readlane( (int)( mine >> 32 ), i ) << 32 | (uint32_t)__builtin_amdgcn_readlane( (int)(uint32_t)mine, i );
-      rank += other > mine || ( other == mine && i < lane );
-    }
-    const uint64_t which = __builtin_amdgcn_ballot_w64( rank == n_top - 1 );
-    const int at = __builtin_ctzll( which );
-    reach = (uint64_t)__builtin_amdgcn_readlane( (int)( mine >> 32 ), at ) << 32 | (uint32_t)__builtin_amdgcn_readlane( (int)(uint32_t)mine, at );
-  }
+  const float wave_s = wave_sum( ( s4[0] + s4[1] ) + ( s4[2] + s4[3] ) ), wave_t = wave_sum( ( t4[0] + t4[1] ) + ( t4[2] + t4[3] ) );
   if ( lane == 0 ) {
-    s_sums[wave] = z;
-    s_reach[wave] = reach;
+    s_sums[wave] = make_float2( wave_s, wave_t );
+  }
+  if ( n_top != 0 ) {
+    // the middle one of the waves' values: as many are larger, or equal and in front
+    const float mine = s_reach[lane % WAVES];
+    uint32_t rank = 0;
+#pragma unroll
+    for ( uint32_t w = 0; w < WAVES; w++ ) {
+      const float other = lane_value( mine, (int)w );
+      rank += other > mine || ( other == mine && w < lane );
+    }
+    const float reach = lane_value( mine, __builtin_ctzll( __builtin_amdgcn_ballot_w64( rank == WAVES / 2 - 1 ) ) );
+    if ( !( best < reach ) ) { // few threads come this far
+#pragma unroll
+      for ( int p = 0; p < PIECES; p++ ) {
+        if ( !( piece_best[p] < reach ) ) {
+#pragma unroll
+          for ( int e = 0; e < V; e++ ) {
+            const float v = to_f32( piece[p].e[e] );
+            const uint32_t i = ( p * THREADS + threadIdx.x ) * V + e;
+            if ( !( v < reach ) && i < n ) { // (NaN comes along: where there is nothing else it is wanted)
+              const uint32_t at = atomicAdd( &s_count, 1u ); // (their order does not matter: each is ranked among all)
+              if ( at < CANDIDATES ) {
+                s_number[at] = number_of( v, i );
+              }
+            }
+          }
+        }
+      }
+    }
   }
   __syncthreads();
-  z = s_sums[0];
-  reach = s_reach[0];
+  float2 total = s_sums[0];
+#pragma unroll
   for ( int w = 1; w < WAVES; w++ ) {
-    z = join( z, s_sums[w] );
-    reach = max( reach, s_reach[w] );
+    total.x += s_sums[w].x;
+    total.y += s_sums[w].y;
   }
+  const Sums z = sums_of( max_m, m, c, total.x, total.y );
   const uint64_t part = row * gridDim.x + blockIdx.x;
   if ( threadIdx.x == 0 ) {
     if ( gridDim.x == 1 ) {
@@ -184,39 +249,21 @@ __global__ __launch_bounds__( THREADS ) void logprob_kernel( Outputs o, const T*
   if ( n_top == 0 ) {
     return;
   }
-  const float max_m = z.m == -INFINITY ? 0.0f : z.m, log_s = logf( z.s );
+  const float log_s = logf( z.s );
   auto put = [&]( uint32_t rank, uint64_t number ) {
     if ( gridDim.x != 1 ) {
       tops[part * n_top + rank] = number == 0 ? 0 : ( number & 0xffffffff00000000ull ) | (uint32_t)~( index_of( number ) + c0 );
     } else {
       o.top_ids[row * n_top + rank] = index_of( number );
-      o.top_logprobs[row * n_top + rank] = ( value_of( number ) - max_m ) - log_s;
+      o.top_logprobs[row * n_top + rank] = ( value_of( number ) - m ) - log_s;
     }
   };
-  const float reach_value = value_of( reach );
-#pragma unroll
-  for ( int p = 0; p < PIECES; p++ ) {
-#pragma unroll
-    for ( int e = 0; e < V; e++ ) {
-      const float v = to_f32( piece[p].e[e] );
-      if ( !( v < reach_value ) ) { // few come this far
-        const uint32_t i = ( p * THREADS + threadIdx.x ) * V + e;
-        const uint64_t number = number_of( v, i );
-        if ( i < n && number >= reach ) {
-          const uint32_t at = atomicAdd( &s_count, 1u ); // (their order does not matter: each is ranked among all)
-          if ( at < CANDIDATES ) {
-            s_number[at] = number;
-          }
-        }
-      }
-    }
-  }
-  __syncthreads();
   const uint32_t count = s_count;
   if ( count <= CANDIDATES ) {
     for ( uint32_t i = threadIdx.x; i < count; i += THREADS ) {
       const uint64_t number = s_number[i];
       uint32_t rank = 0;
+#pragma unroll 8
       for ( uint32_t k = 0; k < count; k++ ) {
         rank += s_number[k] > number;
       }
@@ -309,13 +356,13 @@ struct LogprobPlan
   uint64_t bytes;
 };
 
-// columns of a piece differ with the type; the workspace has to serve every type, so the parts are those of fp32 pieces of four
+// A row is one part while it fits the registers of a work-group: more parts for few rows take the launch that joins them, which costs what they save (1 row of 32000
+// fp32 values, 5 alternatives: one part 10.8 us, 7 parts and the join 10.4; 64 alternatives 15 and 20).
 LogprobPlan plan_logprobs( uint64_t rows, uint64_t vocab, uint32_t n_top )
 {
   LogprobPlan p {};
   constexpr uint64_t MOST = 32768; // columns of a part at most
-  const uint64_t wanted = std::max<uint64_t>( 1, (uint64_t)cu_count() / std::max<uint64_t>( rows, 1 ) );  // few rows: a part for every CU
-  uint64_t parts = std::max<uint64_t>( ( vocab + MOST - 1 ) / MOST, std::min<uint64_t>( wanted, std::min<uint64_t>( vocab / 4096, 16 ) ) );
+  const uint64_t parts = ( vocab + MOST - 1 ) / MOST;
   p.per_part = (uint32_t)( ( ( vocab + parts - 1 ) / parts + 7 ) / 8 * 8 );
   p.parts = (uint32_t)( ( vocab + p.per_part - 1 ) / p.per_part );
   p.bytes = p.parts == 1 ? 0 : rows * p.parts * ( ( n_top + 2 ) * sizeof( uint64_t ) );
