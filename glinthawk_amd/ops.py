@@ -7,6 +7,7 @@ one call into libglint_hip.so.  Names follow the reference's op names
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional, Sequence
 
 import torch
@@ -426,18 +427,22 @@ def convert(dst: torch.Tensor, src: torch.Tensor, n: int) -> None:
 
 
 # ---- a cache in pages -----------------------------------------------------------------------------
-def _same_device(device, **tensors) -> None:
-    """An op's tensors lie on one device, the library's and the current one: a launch on another could not reach them."""
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
+# The checks of these ops are one expression where everything is in order, since a decode step's call is as long as its kernel; what is wrong is found out behind it.
+def _refuse(pool: torch.Tensor, **wanted) -> None:
+    """Says which of the tensors is not (dtype, shape), contiguous and on the pool's device."""
+    for name, (t, dtype, shape) in wanted.items():
+        if t is None:
+            continue
+        if t.device != pool.device:
+            raise ValueError(f"{name} is on {t.device}, not on {pool.device}")
+        if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous {tuple(shape)} of {dtype} expected, got {tuple(t.shape)} of {t.dtype}")
+    raise ValueError("the page table has fewer contexts than the batch, or the rows of the pool are not the shape's")
 
 
-def _u32(t: Optional[torch.Tensor], name: str, *shape) -> None:
-    if t is None:
-        return
-    if t.dtype != torch.int32 or not t.is_contiguous() or (shape and tuple(t.shape) != shape):
-        raise ValueError(f"{name}: a contiguous int32 tensor{' of shape ' + str(shape) if shape else ''} expected, got {tuple(t.shape)} of {t.dtype}")
+@functools.lru_cache(maxsize=None)
+def _shape_ref(shape: Shape):
+    return C.byref(shape.c())
 
 
 def pages(pool: torch.Tensor, table: torch.Tensor) -> GhPages:
@@ -446,93 +451,77 @@ def pages(pool: torch.Tensor, table: torch.Tensor) -> GhPages:
         raise ValueError("the rows of a page lie one behind the other: (pages, tokens, 2 * kv_dim) expected")
     if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous():
         raise ValueError("the table is a contiguous (contexts, entries) int32 tensor")
-    _same_device(pool.device, table=table)
+    if table.device != pool.device:
+        raise ValueError(f"the table is on {table.device}, not on {pool.device}")
     p = GhPages(pool.data_ptr(), pool.stride(0) * pool.element_size(), pool.shape[0], pool.shape[1], table.data_ptr(), table.shape[1])
-    p.tensors = (pool, table)
+    p.pool_tensor, p.table_tensor, p.dtype, p.dt, p.device, p.row, p.contexts = pool, table, pool.dtype, _dt(pool), pool.device, pool.shape[2], table.shape[0]
     return p
-
-
-def _check_paged(p: GhPages, shape: Shape, batch: int, **tensors) -> None:
-    pool, table = p.tensors
-    if pool.shape[2] != 2 * shape.kv_dim:
-        raise ValueError(f"rows of {pool.shape[2]} elements, the shape's have {2 * shape.kv_dim}")
-    if table.shape[0] < batch:
-        raise ValueError(f"a table of {table.shape[0]} contexts for a batch of {batch}")
-    _same_device(pool.device, **tensors)
-    for name in ("q", "xb"):
-        t = tensors[name]
-        if t.dtype != pool.dtype or t.dim() != 2 or t.shape[1] != shape.dim or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous rows of {shape.dim} x {pool.dtype} expected, got {tuple(t.shape)} of {t.dtype}")
-    if tensors["q"].shape != tensors["xb"].shape:
-        raise ValueError("q and xb differ in shape")
 
 
 def page_rows(p: GhPages, first: torch.Tensor, start_pos: Optional[torch.Tensor], n_tokens: int):
     """(addresses of the tokens' cache rows, their positions): the tables kv_append, rope and matmul_qkv_rope_append take."""
-    pool, table = p.tensors
     batch = first.numel() - 1
-    _u32(first, "first")
-    _u32(start_pos, "start_pos", batch)
-    if table.shape[0] < batch:
-        raise ValueError(f"a table of {table.shape[0]} contexts for {batch} sequences")
-    _same_device(pool.device, first=first, start_pos=start_pos)
-    rows = torch.empty(n_tokens, dtype=torch.int64, device=pool.device)
-    pos = torch.empty(n_tokens, dtype=torch.int32, device=pool.device)
-    check(lib().gh_page_rows(C.byref(p), _p(first), _p(start_pos), batch, n_tokens, pool.shape[2] // 2, _p(rows), _p(pos), _dt(pool), _stream()), "gh_page_rows")
+    if not (first.dtype is torch.int32 and first.is_contiguous() and first.device == p.device and p.contexts >= batch
+            and (start_pos is None or (start_pos.dtype is torch.int32 and start_pos.shape == (batch,) and start_pos.is_contiguous() and start_pos.device == p.device))):
+        _refuse(p.pool_tensor, first=(first, torch.int32, (batch + 1,)), start_pos=(start_pos, torch.int32, (batch,)))
+    rows = torch.empty(n_tokens, dtype=torch.int64, device=p.device)
+    pos = torch.empty(n_tokens, dtype=torch.int32, device=p.device)
+    check(lib().gh_page_rows(C.byref(p), first.data_ptr(), _p(start_pos), batch, n_tokens, p.row // 2, _p(rows), _p(pos), p.dt, _stream()), "gh_page_rows")
     return rows, pos
 
 
 def attn_decode_paged_workspace(batch: int, max_length: int, shape: Shape, dtype: torch.dtype) -> int:
-    s = shape.c()
-    return int(lib().gh_attn_decode_paged_workspace(batch, max_length, C.byref(s), _dt(torch.empty(0, dtype=dtype))))
+    """Bytes that serve every call of at most so many contexts and keys."""
+    return int(lib().gh_attn_decode_paged_workspace(batch, max_length, _shape_ref(shape), _dt(torch.empty(0, dtype=dtype))))
 
 
 def attn_decode_paged(q: torch.Tensor, p: GhPages, lengths: torch.Tensor, xb: torch.Tensor, max_length: int, shape: Shape,
                       workspace: Optional[torch.Tensor] = None) -> None:
-    s = shape.c()
     batch = q.shape[0]
-    _u32(lengths, "lengths", batch)
-    _check_paged(p, shape, batch, q=q, xb=xb, lengths=lengths, workspace=workspace)
+    if not (q.dtype is p.dtype and xb.dtype is p.dtype and lengths.dtype is torch.int32 and q.shape == (batch, shape.dim) and xb.shape == q.shape and lengths.shape == (batch,)
+            and q.is_contiguous() and xb.is_contiguous() and lengths.is_contiguous() and q.device == p.device and xb.device == p.device and lengths.device == p.device
+            and (workspace is None or (workspace.device == p.device and workspace.is_contiguous())) and p.contexts >= batch and p.row == 2 * shape.kv_dim):
+        _refuse(p.pool_tensor, q=(q, p.dtype, (batch, shape.dim)), xb=(xb, p.dtype, (batch, shape.dim)), lengths=(lengths, torch.int32, (batch,)),
+                workspace=(workspace, None if workspace is None else workspace.dtype, () if workspace is None else workspace.shape))
     if workspace is None:
         workspace = torch.empty(attn_decode_paged_workspace(batch, max_length, shape, q.dtype), dtype=torch.uint8, device=q.device)
-    check(lib().gh_attn_decode_paged(_p(q), C.byref(p), _p(lengths), _p(xb), batch, max_length, C.byref(s), _dt(q), _p(workspace),
-                                     workspace.numel() * workspace.element_size(), _stream()), "gh_attn_decode_paged")
+    check(lib().gh_attn_decode_paged(q.data_ptr(), C.byref(p), lengths.data_ptr(), xb.data_ptr(), batch, max_length, _shape_ref(shape), p.dt, workspace.data_ptr(),
+                                     workspace.nbytes, _stream()), "gh_attn_decode_paged")
 
 
 def attn_packed_workspace(batch: int, n_tokens: int, max_keys: int, shape: Shape, dtype: torch.dtype) -> int:
-    s = shape.c()
-    return int(lib().gh_attn_packed_workspace(batch, n_tokens, max_keys, C.byref(s), _dt(torch.empty(0, dtype=dtype))))
+    """Bytes that serve every call of at most so many sequences, tokens and keys."""
+    return int(lib().gh_attn_packed_workspace(batch, n_tokens, max_keys, _shape_ref(shape), _dt(torch.empty(0, dtype=dtype))))
 
 
 def attn_packed(q: torch.Tensor, p: GhPages, first: torch.Tensor, start_pos: Optional[torch.Tensor], xb: torch.Tensor, max_keys: int, shape: Shape,
                 workspace: Optional[torch.Tensor] = None) -> None:
     """first: (sequences + 1) int32, where each sequence's tokens begin in q and xb; start_pos: (sequences) int32 or None."""
-    s = shape.c()
-    batch = first.numel() - 1
-    _u32(first, "first")
-    _u32(start_pos, "start_pos", batch)
-    _check_paged(p, shape, batch, q=q, xb=xb, first=first, start_pos=start_pos, workspace=workspace)
+    tokens, batch = q.shape[0], first.numel() - 1
+    if not (q.dtype is p.dtype and xb.dtype is p.dtype and first.dtype is torch.int32 and q.shape == (tokens, shape.dim) and xb.shape == q.shape and first.shape == (batch + 1,)
+            and q.is_contiguous() and xb.is_contiguous() and first.is_contiguous() and q.device == p.device and xb.device == p.device and first.device == p.device
+            and (start_pos is None or (start_pos.dtype is torch.int32 and start_pos.shape == (batch,) and start_pos.is_contiguous() and start_pos.device == p.device))
+            and (workspace is None or (workspace.device == p.device and workspace.is_contiguous())) and p.contexts >= batch and p.row == 2 * shape.kv_dim):
+        _refuse(p.pool_tensor, q=(q, p.dtype, (tokens, shape.dim)), xb=(xb, p.dtype, (tokens, shape.dim)), first=(first, torch.int32, (batch + 1,)),
+                start_pos=(start_pos, torch.int32, (batch,)), workspace=(workspace, None if workspace is None else workspace.dtype, () if workspace is None else workspace.shape))
     if workspace is None:
-        workspace = torch.empty(attn_packed_workspace(batch, q.shape[0], max_keys, shape, q.dtype), dtype=torch.uint8, device=q.device)
-    check(lib().gh_attn_packed(_p(q), C.byref(p), _p(first), _p(start_pos), _p(xb), batch, q.shape[0], max_keys, C.byref(s), _dt(q), _p(workspace),
-                               workspace.numel() * workspace.element_size(), _stream()), "gh_attn_packed")
+        workspace = torch.empty(attn_packed_workspace(batch, tokens, max_keys, shape, q.dtype), dtype=torch.uint8, device=q.device)
+    check(lib().gh_attn_packed(q.data_ptr(), C.byref(p), first.data_ptr(), _p(start_pos), xb.data_ptr(), batch, tokens, max_keys, _shape_ref(shape), p.dt,
+                               workspace.data_ptr(), workspace.nbytes, _stream()), "gh_attn_packed")
 
 
 def copy_pages(pool: torch.Tensor, pairs) -> None:
     """pool: (layers, pages, tokens, elements) or (pages, tokens, elements); pairs: (n, 2) of (source, destination), an int32 tensor on the device or a
     sequence of pairs in host memory, which is checked."""
-    layered = pool if pool.dim() == 4 else pool[None]
-    if layered.dim() != 4 or layered.stride(3) != 1 or layered.stride(2) != layered.shape[3]:
+    stride, (layers, n_pages, tokens, row) = pool.stride(), (pool.shape if pool.dim() == 4 else (1, *pool.shape) if pool.dim() == 3 else (0, 0, 0, 0))
+    if not n_pages or stride[-1] != 1 or stride[-2] != row:
         raise ValueError("the rows of a page lie one behind the other: ([layers,] pages, tokens, elements) expected")
     size = pool.element_size()
-    layers, n_pages, tokens, row = layered.shape
-    common = layered.data_ptr(), layered.stride(1) * size, tokens * row * size, n_pages, layers, layered.stride(0) * size
+    common = pool.data_ptr(), stride[-3] * size, tokens * row * size, n_pages, layers, stride[0] * size if len(stride) == 4 else 0
     if isinstance(pairs, torch.Tensor):
-        if pairs.dim() != 2 or pairs.shape[1] != 2:
-            raise ValueError(f"pairs: (n, 2) expected, got {tuple(pairs.shape)}")
-        _u32(pairs, "pairs")
-        _same_device(pool.device, pairs=pairs)
-        check(lib().gh_copy_pages(*common, _p(pairs), pairs.shape[0], _stream()), "gh_copy_pages")
+        if not (pairs.dtype is torch.int32 and pairs.dim() == 2 and pairs.shape[1] == 2 and pairs.is_contiguous() and pairs.device == pool.device):
+            _refuse(pool, pairs=(pairs, torch.int32, (pairs.shape[0] if pairs.dim() else 0, 2)))
+        check(lib().gh_copy_pages(*common, pairs.data_ptr(), pairs.shape[0], _stream()), "gh_copy_pages")
     else:
         flat = [int(v) for pair in pairs for v in pair]
         check(lib().gh_copy_pages_host(*common, host_u32_array(flat), len(flat) // 2, _stream()), "gh_copy_pages_host")
@@ -546,16 +535,17 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, n_top: int = 0, w
     """(log probability of each row's token, entropy, (rows, n_top) indices of the largest values, their log probabilities)"""
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise ValueError("rows of logits lie with their values one behind the other")
-    rows, vocab = logits.shape
-    _u32(tokens, "tokens", rows)
-    _same_device(logits.device, tokens=tokens, workspace=workspace)
+    (rows, vocab), device = logits.shape, logits.device
+    if not (tokens.dtype is torch.int32 and tokens.shape == (rows,) and tokens.is_contiguous() and tokens.device == device
+            and (workspace is None or (workspace.device == device and workspace.is_contiguous()))):
+        _refuse(logits, tokens=(tokens, torch.int32, (rows,)), workspace=(workspace, None if workspace is None else workspace.dtype, () if workspace is None else workspace.shape))
     if workspace is None:
-        workspace = torch.empty(token_logprobs_workspace(rows, vocab, n_top), dtype=torch.uint8, device=logits.device)
-    given, entropy = torch.empty((2, rows), dtype=torch.float32, device=logits.device).unbind()
-    ids = torch.empty((rows, n_top), dtype=torch.int32, device=logits.device)
-    values = torch.empty((rows, n_top), dtype=torch.float32, device=logits.device)
-    check(lib().gh_token_logprobs(_p(given), _p(entropy), _p(ids), _p(values), logits.data_ptr(), logits.stride(0), _p(tokens), vocab, rows, n_top, _dt(logits),
-                                  _p(workspace), workspace.numel() * workspace.element_size(), _stream()), "gh_token_logprobs")
+        workspace = torch.empty(token_logprobs_workspace(rows, vocab, n_top), dtype=torch.uint8, device=device)
+    given, entropy = torch.empty(rows, dtype=torch.float32, device=device), torch.empty(rows, dtype=torch.float32, device=device)
+    ids = torch.empty((rows, n_top), dtype=torch.int32, device=device)
+    values = torch.empty((rows, n_top), dtype=torch.float32, device=device)
+    check(lib().gh_token_logprobs(given.data_ptr(), entropy.data_ptr(), ids.data_ptr(), values.data_ptr(), logits.data_ptr(), logits.stride(0), tokens.data_ptr(), vocab, rows,
+                                  n_top, _dt(logits), workspace.data_ptr(), workspace.nbytes, _stream()), "gh_token_logprobs")
     return given, entropy, ids, values
 
 
