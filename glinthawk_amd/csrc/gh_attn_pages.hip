@@ -364,7 +364,7 @@ __global__ __launch_bounds__( 256 ) void attn_pages_f32_kernel( const T* __restr
 }
 
 // =================================================================================================
-// decode, 16-bit heads of 8 CH elements and fewer: wave <-> (context, kv head, 16 columns, run of keys)
+// decode, heads of up to CH chunks of 16 bytes: wave <-> (context, kv head, 16 columns, run of keys)
 //
 // Bound by the bytes of the cache.  A wave goes through stages of 32 keys on its own: their K and V rows go from memory straight to its part of LDS, two stages deep,
 // so that a stage (16 KB at 128 elements) is always on its way while one is computed.  Rows behind the keys, and chunks behind a smaller head, lie outside the
@@ -374,6 +374,7 @@ __global__ __launch_bounds__( 256 ) void attn_pages_f32_kernel( const T* __restr
 //                   lanes take those keys of one dim with transposing LDS reads
 // 16-byte chunks of a row are swizzled by the row (in the address a lane fetches) so that both reads touch every bank once.
 // The weights are rounded to the storage type for the second product, as the matrix units take them; the sum takes them rounded too.
+// fp32: both products 16 x 16 x 4, a chunk of K being four of its steps, weights as they are, and V read value by value; 16 keys a stage above 64 elements.
 // W waves of a work-group take the stages of one run in turns and are joined through LDS.
 // =================================================================================================
 typedef __attribute__( ( address_space( 3 ) ) ) void* lds_ptr;
@@ -402,12 +403,49 @@ __device__ __forceinline__ float rounded( float v )
   return to_f32( from_f32<E>( v ) );
 }
 
+template<typename E>
+struct ChunkOf // 16 bytes as the matrix instructions take them
+{
+  using type = typename Mfma<E>::x8;
+};
+template<>
+struct ChunkOf<float>
+{
+  using type = mfma_f32x4;
+};
+
+// four neighbouring values of a row, aligned to them
+template<typename E>
+__device__ __forceinline__ void store4( E* to, float a, float b, float c, float d )
+{
+  if constexpr ( sizeof( E ) == 4 ) {
+    *reinterpret_cast<float4*>( to ) = make_float4( a, b, c, d );
+  } else {
+    *reinterpret_cast<uint2*>( to ) = make_uint2( rounded_pair<E>( a, b ), rounded_pair<E>( c, d ) );
+  }
+}
+
 // LDS reads of a stage, written out, each block with its waits: the compiler cannot tell the tiles that a read may take from the ones on their way, and would wait
 // for all of them.
-template<int CH, uint32_t FIRST, uint32_t SECOND, typename X8>
-__device__ __forceinline__ void read_keys( const uint32_t* at, X8 ( &k )[2][CH / 4] )
+template<int CH, uint32_t FIRST, uint32_t SECOND, typename Chunk, uint32_t NU>
+__device__ __forceinline__ void read_keys( const uint32_t* at, Chunk ( &k )[NU][CH / 4] )
 {
-  if constexpr ( CH == 16 ) {
+  if constexpr ( CH == 32 ) {
+    static_assert( NU == 1, "" );
+    asm volatile( "s_waitcnt vmcnt(16)\n\t"
+                  "ds_read_b128 %0, %8 offset:%16\n\t"
+                  "ds_read_b128 %1, %9 offset:%16\n\t"
+                  "ds_read_b128 %2, %10 offset:%16\n\t"
+                  "ds_read_b128 %3, %11 offset:%16\n\t"
+                  "ds_read_b128 %4, %12 offset:%16\n\t"
+                  "ds_read_b128 %5, %13 offset:%16\n\t"
+                  "ds_read_b128 %6, %14 offset:%16\n\t"
+                  "ds_read_b128 %7, %15 offset:%16\n\t"
+                  "s_waitcnt lgkmcnt(0)"
+                  : "=&v"( k[0][0] ), "=&v"( k[0][1] ), "=&v"( k[0][2] ), "=&v"( k[0][3] ), "=&v"( k[0][4] ), "=&v"( k[0][5] ), "=&v"( k[0][6] ), "=&v"( k[0][7] )
+                  : "v"( at[0] ), "v"( at[1] ), "v"( at[2] ), "v"( at[3] ), "v"( at[4] ), "v"( at[5] ), "v"( at[6] ), "v"( at[7] ), "n"( FIRST )
+                  : "memory" );
+  } else if constexpr ( CH == 16 ) {
     asm volatile( "s_waitcnt vmcnt(16)\n\t"
                   "ds_read_b128 %0, %8 offset:%12\n\t"
                   "ds_read_b128 %1, %9 offset:%12\n\t"
@@ -451,16 +489,91 @@ __device__ __forceinline__ void read_values( const uint32_t* at, v4s ( *v )[2] )
                 : "memory" );
 }
 
+// A stage's values as the first operand of O^T += V^T P^T
+template<typename E, uint32_t NB, uint32_t NU>
+struct Values
+{
+  v4s half[NB][2];
+  template<int CH, uint32_t FIRST, uint32_t SECOND>
+  __device__ __forceinline__ void read( const uint32_t* at )
+  {
+#pragma unroll
+    for ( uint32_t n = 0; n < NB; n += 4 ) {
+      read_values<FIRST, SECOND>( at + n, half + n );
+    }
+  }
+  __device__ __forceinline__ void add( const float* p, mfma_f32x4 ( &acc )[NB] ) const
+  {
+    typedef uint32_t u32x4 __attribute__( ( ext_vector_type( 4 ) ) );
+    using X8 = typename Mfma<E>::x8;
+    const X8 pk = __builtin_bit_cast( X8, ( u32x4 { rounded_pair<E>( p[0], p[1] ), rounded_pair<E>( p[2], p[3] ), rounded_pair<E>( p[4], p[5] ), rounded_pair<E>( p[6], p[7] ) } ) );
+#pragma unroll
+    for ( uint32_t n = 0; n < NB; n++ ) {
+      const v8s v = v8s { half[n][0][0], half[n][0][1], half[n][0][2], half[n][0][3], half[n][1][0], half[n][1][1], half[n][1][2], half[n][1][3] };
+      acc[n] = Mfma<E>::k32( __builtin_bit_cast( X8, v ), pk, acc[n] );
+    }
+  }
+};
+// eight values of fp32 rows 16 CH bytes apart: of four rows and the four 16 rows on, or of four rows at two addresses
+template<int CH, uint32_t FIRST, bool TWO>
+__device__ __forceinline__ void read_values_f32( const uint32_t* at, float* v )
+{
+  constexpr uint32_t ROW = CH * 16, NEXT = TWO ? FIRST : FIRST + 16 * ROW;
+  asm volatile( "ds_read_b32 %0, %8 offset:%10\n\t"
+                "ds_read_b32 %1, %8 offset:%11\n\t"
+                "ds_read_b32 %2, %8 offset:%12\n\t"
+                "ds_read_b32 %3, %8 offset:%13\n\t"
+                "ds_read_b32 %4, %9 offset:%14\n\t"
+                "ds_read_b32 %5, %9 offset:%15\n\t"
+                "ds_read_b32 %6, %9 offset:%16\n\t"
+                "ds_read_b32 %7, %9 offset:%17\n\t"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"( v[0] ), "=&v"( v[1] ), "=&v"( v[2] ), "=&v"( v[3] ), "=&v"( v[4] ), "=&v"( v[5] ), "=&v"( v[6] ), "=&v"( v[7] )
+                : "v"( at[0] ), "v"( at[TWO ? 1 : 0] ), "n"( FIRST ), "n"( FIRST + ROW ), "n"( FIRST + 2 * ROW ), "n"( FIRST + 3 * ROW ), "n"( NEXT ), "n"( NEXT + ROW ),
+                  "n"( NEXT + 2 * ROW ), "n"( NEXT + 3 * ROW )
+                : "memory" );
+}
+template<uint32_t NB, uint32_t NU>
+struct Values<float, NB, NU>
+{
+  float v[NB][NU][4];
+  template<int CH, uint32_t FIRST, uint32_t SECOND>
+  __device__ __forceinline__ void read( const uint32_t* at )
+  {
+#pragma unroll
+    for ( uint32_t n = 0; n < NB; n += 3 - NU ) {
+      read_values_f32<CH, FIRST, NU == 1>( at + n, &v[n][0][0] );
+    }
+  }
+  __device__ __forceinline__ void add( const float* p, mfma_f32x4 ( &acc )[NB] ) const
+  {
+#pragma unroll
+    for ( uint32_t u = 0; u < NU; u++ ) {
+#pragma unroll
+      for ( uint32_t i = 0; i < 4; i++ ) {
+#pragma unroll
+        for ( uint32_t n = 0; n < NB; n++ ) {
+          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32( v[n][u][i], p[4 * u + i], acc[n], 0, 0, 0 );
+        }
+      }
+    }
+  }
+};
+
 template<typename E, int CH, int W, int HW>
 __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restrict__ out, const Call& a )
 {
-  constexpr uint32_t KK = CH / 4, NB = CH / 2; // k steps of the scores, blocks of 16 dims
+  constexpr bool F32 = sizeof( E ) == 4;
+  constexpr uint32_t PER = 16 / sizeof( E );                    // elements of a chunk
+  constexpr uint32_t KEYS = F32 && CH == 32 ? 16 : 32;          // of a stage
+  constexpr uint32_t KK = CH / 4, NB = CH * PER / 16;           // chunks of a key that a lane reads, blocks of 16 dims
+  constexpr uint32_t NU = KEYS / 16;
   constexpr uint32_t RPI = 64 / CH;            // rows that a load of the wave fetches
   constexpr uint32_t IPG = 16 / RPI;           // loads for 16 rows of K, or of V
-  using X8 = typename Mfma<E>::x8;
-  constexpr uint32_t TILE = 32 * CH * 16;      // bytes
+  using Chunk = typename ChunkOf<E>::type;
+  constexpr uint32_t TILE = KEYS * CH * 16;    // bytes
   static_assert( W == 1 || HW == 1, "" );
-  __shared__ uint4 s_tiles[W * HW][4][32 * CH]; // of every wave: K of even and of odd stages, V of even and of odd stages
+  __shared__ uint4 s_tiles[W * HW][4][KEYS * CH]; // of every wave: K of even and of odd stages, V of even and of odd stages
 
   const uint32_t wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 ), lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
   Block b;
@@ -476,19 +589,19 @@ __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restri
   const bool ok = col < a.gqa;
   const uint64_t place = (uint64_t)b.row0 * a.n_kv_heads * a.gqa + (uint64_t)b.h * a.gqa + ( ok ? col : 0 );
 
-  uint4( *const tiles )[32 * CH] = s_tiles[wave + hw];
-  X8 qb[KK];
+  uint4( *const tiles )[KEYS * CH] = s_tiles[wave + hw];
+  Chunk qb[KK];
 #pragma unroll
   for ( uint32_t kk = 0; kk < KK; kk++ ) {
-    const uint32_t d = 8 * ( 4 * kk + g4 );
-    qb[kk] = ok && d < a.size ? *reinterpret_cast<const X8*>( q + place * a.size + d ) : X8 { 0, 0, 0, 0, 0, 0, 0, 0 };
+    const uint32_t d = PER * ( 4 * kk + g4 );
+    qb[kk] = ok && d < a.size ? *reinterpret_cast<const Chunk*>( q + place * a.size + d ) : Chunk {};
   }
 
   // a lane's place in the rows of a load: row lane / CH, slot lane % CH, which keeps chunk slot ^ (swizzle of the row)
-  const uint32_t ld_row = lane / CH, ld_slot = lane % CH, chunks = a.size / 8;
-  const uint32_t k_off = b.h * a.size * 2, v_off = ( a.n_kv_heads + b.h ) * a.size * 2;
-  auto k_swizzle = []( uint32_t row ) { return CH == 16 ? row & 15 : ( row >> 1 ) & 7; };
-  auto v_swizzle = []( uint32_t row ) { return CH == 16 ? 2 * ( row & 7 ) : 2 * ( ( row >> 1 ) & 3 ); };
+  const uint32_t ld_row = lane / CH, ld_slot = lane % CH, chunks = a.size / PER;
+  const uint32_t k_off = b.h * a.size * sizeof( E ), v_off = ( a.n_kv_heads + b.h ) * a.size * sizeof( E );
+  auto k_swizzle = []( uint32_t row ) { return CH >= 16 ? row & 15 : ( row >> 1 ) & 7; };
+  auto v_swizzle = []( uint32_t row ) { return F32 ? row & 12 : CH == 16 ? 2 * ( row & 7 ) : 2 * ( ( row >> 1 ) & 3 ); };
   uint32_t k_at[IPG], v_at[IPG];
 #pragma unroll
   for ( uint32_t t = 0; t < IPG; t++ ) {
@@ -497,23 +610,23 @@ __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restri
     v_at[t] = vc < chunks ? row * a.pages.row_bytes + v_off + 16 * vc : 0x80000000u;
   }
 
-  const uint32_t n_stages = ( k_end - k_begin + 31 ) / 32, n_mine = n_stages > wave ? ( n_stages - wave + W - 1 ) / W : 0;
+  const uint32_t n_stages = ( k_end - k_begin + KEYS - 1 ) / KEYS, n_mine = n_stages > wave ? ( n_stages - wave + W - 1 ) / W : 0;
   // Page numbers are read by scalar loads one stage before they are needed: vector loads would be counted with the loads to LDS, and waiting for one would be
   // waiting for those.
   typedef const uint32_t __attribute__( ( address_space( 4 ) ) ) * scalar_ptr;
   const scalar_ptr table = (scalar_ptr)( reinterpret_cast<uintptr_t>( a.pages.table + (uint64_t)b.seq * a.pages.table_stride ) );
-  uint32_t id[2];
+  uint32_t id[NU];
   auto look_up = [&]( uint32_t stage ) __attribute__( ( always_inline ) ) {
 #pragma unroll
-    for ( uint32_t u = 0; u < 2; u++ ) {
-      id[u] = table[min( k_begin + 32 * ( stage * W + wave ) + 16 * u, k_end - 1 ) >> a.pages.shift];
+    for ( uint32_t u = 0; u < NU; u++ ) {
+      id[u] = table[min( k_begin + KEYS * ( stage * W + wave ) + 16 * u, k_end - 1 ) >> a.pages.shift];
     }
   };
-  __amdgpu_buffer_rsrc_t rsrc[2];
+  __amdgpu_buffer_rsrc_t rsrc[NU];
   auto describe = [&]( uint32_t stage ) __attribute__( ( always_inline ) ) {
 #pragma unroll
-    for ( uint32_t u = 0; u < 2; u++ ) {
-      const uint32_t key = k_begin + 32 * ( stage * W + wave ) + 16 * u;
+    for ( uint32_t u = 0; u < NU; u++ ) {
+      const uint32_t key = k_begin + KEYS * ( stage * W + wave ) + 16 * u;
       const char* base = a.pages.pool + min( id[u], a.pages.last ) * a.pages.stride + (uint64_t)( key & ( ( 1u << a.pages.shift ) - 1 ) ) * a.pages.row_bytes;
       const uint32_t rows = key < k_end ? min( k_end - key, 16u ) : 0u;
       rsrc[u] = __builtin_amdgcn_make_buffer_rsrc( const_cast<char*>( base ), 0, (int)( rows * a.pages.row_bytes ), 0x00020000 );
@@ -522,7 +635,7 @@ __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restri
   };
   auto fetch = [&]( uint4* tile, const uint32_t( &at )[IPG] ) __attribute__( ( always_inline ) ) {
 #pragma unroll
-    for ( uint32_t u = 0; u < 2; u++ ) {
+    for ( uint32_t u = 0; u < NU; u++ ) {
 #pragma unroll
       for ( uint32_t t = 0; t < IPG; t++ ) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds( rsrc[u], (lds_ptr)( tile + ( 16 * u + RPI * t ) * CH ), 16, at[t], 0, 0, 2 ); // (read once: streaming)
@@ -537,46 +650,57 @@ __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restri
   }
   float m = -INFINITY, l = 0.0f; // l: of this lane's keys
 
-  // K: row c and row 16 + c, chunk 4 kk + g4.  V, transposing: lane 4 e + p of 16 points at dims 4 p .. 4 p + 3 of key 4 g4 + e and receives
-  // one dim of the four keys.
+  // K: row c (and row 16 + c), chunk 4 kk + g4.  V in 16 bits, transposing: lane 4 e + p of 16 points at dims 4 p .. 4 p + 3 of key 4 g4 + e and receives
+  // one dim of the four keys.  V in fp32: dim c of a block, of keys 4 g4 + i.
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)&tiles[0][0];
-  const uint32_t tr_row = 4 * g4 + ( c >> 2 ), tr_at = tr_row * CH * 16 + ( ( ( c & 3 ) >> 1 ) ^ v_swizzle( tr_row ) ) * 16 + ( c & 1 ) * 8;
   uint32_t k_lds[KK], v_lds[NB];
 #pragma unroll
   for ( uint32_t kk = 0; kk < KK; kk++ ) {
     k_lds[kk] = lds0 + c * CH * 16 + ( ( 4 * kk + g4 ) ^ k_swizzle( c ) ) * 16;
   }
+  const uint32_t tr_row = 4 * g4 + ( c >> 2 ), tr_at = tr_row * CH * 16 + ( ( ( c & 3 ) >> 1 ) ^ v_swizzle( tr_row ) ) * 16 + ( c & 1 ) * 8;
 #pragma unroll
   for ( uint32_t n = 0; n < NB; n++ ) {
-    v_lds[n] = lds0 + ( tr_at ^ ( 32 * n ) );
+    v_lds[n] = lds0 + ( F32 ? 4 * g4 * CH * 16 + ( ( 4 * n + ( c >> 2 ) ) ^ ( 4 * g4 ) ) * 16 + ( c & 3 ) * 4 : tr_at ^ ( 32 * n ) );
   }
   // buffer: 0 or 1, j % 2
   auto stage = [&]( uint32_t j, auto buffer ) __attribute__( ( always_inline ) ) {
     constexpr uint32_t B = decltype( buffer )::value, K0 = B * TILE, K1 = K0 + TILE / 2, V0 = ( 2 + B ) * TILE, V1 = V0 + TILE / 2;
     uint4* const kt = tiles[B];
     uint4* const vt = tiles[2 + B];
-    X8 kf[2][KK];
-    read_keys<CH, K0, K1>( k_lds, kf ); // all but the 4 IPG loads of stage j + 1 have landed
+    Chunk kf[NU][KK];
+    read_keys<CH, K0, K1>( k_lds, kf ); // all but the 2 NU IPG loads of stage j + 1 have landed
     __builtin_amdgcn_sched_barrier( 0 );
     describe( j + 2 );
     fetch( kt, k_at ); // the tile has been read
-    mfma_f32x4 st[2];
+    mfma_f32x4 st[NU];
 #pragma unroll
-    for ( uint32_t u = 0; u < 2; u++ ) {
+    for ( uint32_t u = 0; u < NU; u++ ) {
       st[u] = mfma_f32x4 { 0, 0, 0, 0 };
 #pragma unroll
       for ( uint32_t kk = 0; kk < KK; kk++ ) {
-        st[u] = Mfma<E>::k32( kf[u][kk], qb[kk], st[u] );
+        if constexpr ( F32 ) {
+#pragma unroll
+          for ( int e = 0; e < 4; e++ ) {
+            st[u] = __builtin_amdgcn_mfma_f32_16x16x4f32( kf[u][kk][e], qb[kk][e], st[u], 0, 0, 0 );
+          }
+        } else {
+          st[u] = Mfma<E>::k32( kf[u][kk], qb[kk], st[u] );
+        }
       }
     }
-    const uint32_t key0 = k_begin + 32 * ( j * W + wave );
-    if ( key0 + 32 > k_end ) {
+    const uint32_t key0 = k_begin + KEYS * ( j * W + wave );
+    if ( key0 + KEYS > k_end ) {
 #pragma unroll
-      for ( int e = 0; e < 8; e++ ) {
+      for ( uint32_t e = 0; e < 4 * NU; e++ ) {
         st[e >> 2][e & 3] = key0 + 16 * ( e >> 2 ) + 4 * g4 + ( e & 3 ) < k_end ? st[e >> 2][e & 3] : -INFINITY;
       }
     }
-    float mx = fmaxf( fmaxf( fmaxf( st[0][0], st[0][1] ), fmaxf( st[0][2], st[0][3] ) ), fmaxf( fmaxf( st[1][0], st[1][1] ), fmaxf( st[1][2], st[1][3] ) ) );
+    float mx = -INFINITY;
+#pragma unroll
+    for ( uint32_t u = 0; u < NU; u++ ) {
+      mx = fmaxf( mx, fmaxf( fmaxf( st[u][0], st[u][1] ), fmaxf( st[u][2], st[u][3] ) ) );
+    }
     mx = column_max( mx ) * a.scale_log2e;
     if ( __builtin_amdgcn_ballot_w64( mx > m + LAZY ) != 0 ) {
       const float m_new = fmaxf( m, mx ), alpha = m_new == -INFINITY ? 1.0f : fast_exp2( m - m_new );
@@ -588,32 +712,19 @@ __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restri
       }
     }
     const float ms = m == -INFINITY ? 0.0f : m;
-    float p[8];
+    float p[4 * NU], sum[2] = { 0, 0 };
 #pragma unroll
-    for ( int e = 0; e < 8; e++ ) {
+    for ( uint32_t e = 0; e < 4 * NU; e++ ) {
       p[e] = fast_exp2( __builtin_fmaf( st[e >> 2][e & 3], a.scale_log2e, -ms ) );
-    }
-    typedef uint32_t u32x4 __attribute__( ( ext_vector_type( 4 ) ) );
-    const X8 pk = __builtin_bit_cast( X8, ( u32x4 { rounded_pair<E>( p[0], p[1] ), rounded_pair<E>( p[2], p[3] ), rounded_pair<E>( p[4], p[5] ), rounded_pair<E>( p[6], p[7] ) } ) );
-    float sum[2] = { 0, 0 };
-#pragma unroll
-    for ( int e = 0; e < 8; e++ ) {
-      sum[e & 1] += (float)pk[e];
+      sum[e & 1] += rounded<E>( p[e] );
     }
     l += sum[0] + sum[1];
-    v4s half[NB][2];
-#pragma unroll
-    for ( uint32_t n = 0; n < NB; n += 4 ) {
-      read_values<V0, V1>( v_lds + n, half + n );
-    }
+    Values<E, NB, NU> v;
+    v.template read<CH, V0, V1>( v_lds );
     __builtin_amdgcn_sched_barrier( 0 );
     fetch( vt, v_at );
     __builtin_amdgcn_sched_barrier( 0 );
-#pragma unroll
-    for ( uint32_t n = 0; n < NB; n++ ) {
-      const v8s v = v8s { half[n][0][0], half[n][0][1], half[n][0][2], half[n][0][3], half[n][1][0], half[n][1][1], half[n][1][2], half[n][1][3] };
-      acc[n] = Mfma<E>::k32( __builtin_bit_cast( X8, v ), pk, acc[n] );
-    }
+    v.add( p, acc );
   };
 
   if ( n_mine != 0 ) {
@@ -694,7 +805,7 @@ __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restri
       if ( a.splits > 1 ) {
         *reinterpret_cast<mfma_f32x4*>( a.part_out + slot * a.size + d ) = acc[n];
       } else {
-        *reinterpret_cast<uint2*>( out + place * a.size + d ) = make_uint2( rounded_pair<E>( acc[n][0] * inv, acc[n][1] * inv ), rounded_pair<E>( acc[n][2] * inv, acc[n][3] * inv ) );
+        store4( out + place * a.size + d, acc[n][0] * inv, acc[n][1] * inv, acc[n][2] * inv, acc[n][3] * inv );
       }
     }
   }
@@ -1129,35 +1240,36 @@ struct Plan
 {
   uint32_t blocks, splits, chunk; // blocks: grid x
   uint32_t n_blocks;
-  uint32_t waves; // of a work-group of the 16-bit kernel; 0: the fp32 tile kernel
+  uint32_t waves; // of a work-group; 0: the kernel that takes everything
   uint64_t bytes;
 };
 
 // The 16-bit kernels take heads made of 16-byte chunks, runs of 16 keys in one page, and everything aligned to 16 bytes.
-bool takes16( const gh_shape* s, gh_dtype dt )
+bool takes_tiles( const gh_shape* s, gh_dtype dt, bool decode )
 {
-  return dt != GH_F32 && s->head_size % 8 == 0 && s->head_size <= 128;
+  return dt == GH_F32 ? decode && s->head_size % 4 == 0 && s->head_size <= 128 : s->head_size % 8 == 0 && s->head_size <= 128;
 }
 
 constexpr uint64_t MOST_PARTS = 65536; // of (query row, head, split) that leave partial results
 
 // How a call is cut.  Splits are whole numbers of 64 keys.
-Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, const gh_shape* s, bool tiles16 )
+Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, const gh_shape* s, gh_dtype dt, bool tiles )
 {
   Plan p {};
-  const uint32_t cols = decode ? 16 : tiles16 ? 128 : 64;
+  const uint32_t cols = decode ? 16 : tiles ? 128 : 64;
   p.n_blocks = decode ? ( s->gqa_size + cols - 1 ) / cols : 0;
   const uint64_t blocks = decode ? batch * p.n_blocks : std::min<uint64_t>( ( rows * s->gqa_size + cols - 1 ) / cols + batch, rows * s->gqa_size );
   p.blocks = (uint32_t)blocks;
-  if ( decode && tiles16 ) {
-    // Microseconds as measured on MI355X.  A stage of 32 keys takes a wave on its own 0.75, the four waves of a work-group 1.5, and 2.4 where the waves that fit
-    // (four a CU at 128 elements) share the memory's rate; a round of work-groups takes 2 to begin and end; a split adds a launch (4) and 8 bytes an element
+  if ( decode && tiles ) {
+    // Microseconds as measured on MI355X.  A stage of 16 KB takes a wave on its own 0.75, the four waves of a work-group 1.5, and 2.4 where the waves that fit
+    // (four a CU, eight of 16-bit heads up to 64) share the memory's rate; a round of work-groups takes 2 to begin and end; a split adds a launch (4) and 8 bytes an element
     // that go out and come back at 3 TB/s.  Where lengths differ the launch ends on the longest runs: a tenth of a wave's stages.
     // Measured, GQA heads (8 of 8 queries) in f16, us: 1 context of 301 keys, 4 waves 7.0, splits of 64 8.8 | 1 x 4096, 4 waves unsplit 39, splits of 64 10.8 |
     // 16 x 500, 4 waves 9.8, one wave 15.1 | 64 x 4096, splits of 2048 167, of 512 185, of 64 261 | 256 x 1000, one wave 162, 4 waves 177
     // 32 heads of one query: 8 x 2000, 4 waves 42, one wave 48 | 3 x 30000, splits of 1024 233, of 128 248, 4 waves unsplit 269
     const uint64_t streams = batch * p.n_blocks * s->n_kv_heads;
-    const double slots = 4.0 * cu_count() * ( s->head_size <= 64 ? 2 : 1 );
+    const double slots = 4.0 * cu_count() * ( dt != GH_F32 && s->head_size <= 64 ? 2 : 1 );
+    const uint32_t stage = dt == GH_F32 && s->head_size > 64 ? 16 : 32; // keys
     double best = 0;
     for ( uint32_t waves = 1; waves <= 4; waves += 3 ) {
       for ( uint32_t chunk = 64; chunk != 0; chunk = chunk >= max_keys ? 0 : 2 * chunk ) {
@@ -1165,7 +1277,7 @@ Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, c
         if ( splits > 65535 || ( splits > 1 && rows * s->n_heads * splits > MOST_PARTS ) ) {
           continue;
         }
-        const double stages = (double)( ( std::min( chunk, max_keys ) + 32 * waves - 1 ) / ( 32 * waves ) ), load = (double)( streams * splits * waves ) / slots;
+        const double stages = (double)( ( std::min( chunk, max_keys ) + stage * waves - 1 ) / ( stage * waves ) ), load = (double)( streams * splits * waves ) / slots;
         const double alone = waves == 1 ? 0.75 : 1.5, full = std::max( alone, 2.4 * std::min( 1.0, load ) );
         double us = stages * std::max( alone, 2.4 * load ) + 0.1 * stages * full + 2.0 * std::max( 1.0, load );
         if ( splits > 1 ) {
@@ -1183,9 +1295,9 @@ Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, c
     return p;
   }
   // as many splits as bring the launch to four work-groups a CU (two of the 16-bit kernel), of at least 256 keys
-  const uint64_t groups = blocks * s->n_kv_heads, wanted = ( tiles16 ? 2ull : 4ull ) * (uint64_t)cu_count();
+  const uint64_t groups = blocks * s->n_kv_heads, wanted = ( tiles ? 2ull : 4ull ) * (uint64_t)cu_count();
   const uint64_t splits = std::max<uint64_t>( 1, std::min( { wanted / groups, (uint64_t)( max_keys + 255 ) / 256, MOST_PARTS / ( rows * s->n_heads ) } ) );
-  p.waves = tiles16 ? 4 : 0;
+  p.waves = tiles ? 4 : 0;
   p.chunk = (uint32_t)( ( ( max_keys + splits - 1 ) / splits + 63 ) / 64 * 64 );
   p.splits = ( max_keys + p.chunk - 1 ) / p.chunk;
   p.bytes = p.splits == 1 ? 0 : rows * s->n_heads * p.splits * ( s->head_size + 2 ) * sizeof( float );
@@ -1220,7 +1332,7 @@ void launch_f32( const Plan& p, const Call& a, const void* q, void* out, hipStre
 }
 
 template<typename E>
-void launch_decode16( const Plan& p, const Call& a, const void* q, void* out, hipStream_t st )
+void launch_decode_tiles( const Plan& p, const Call& a, const void* q, void* out, hipStream_t st )
 {
   const E* tq = static_cast<const E*>( q );
   E* to = static_cast<E*>( out );
@@ -1240,10 +1352,11 @@ void launch_decode16( const Plan& p, const Call& a, const void* q, void* out, hi
       go( chunks, one, one );
     }
   };
+  constexpr int NARROW = 4 * sizeof( E ); // chunks of 64 elements
   if ( a.size <= 64 ) {
-    sizes( std::integral_constant<int, 8> {} );
+    sizes( std::integral_constant<int, NARROW> {} );
   } else {
-    sizes( std::integral_constant<int, 16> {} );
+    sizes( std::integral_constant<int, 2 * NARROW> {} );
   }
 }
 
@@ -1261,16 +1374,12 @@ void launch_packed16( const Plan& p, const Call& a, const void* q, void* out, hi
 template<typename T, bool DECODE>
 int launch( const Plan& p, const Call& a, const void* q, void* out, uint64_t rows, hipStream_t st )
 {
-  if constexpr ( sizeof( T ) == 2 ) {
-    if ( p.waves != 0 && DECODE ) {
-      launch_decode16<T>( p, a, q, out, st );
-    } else if ( p.waves != 0 ) {
-      launch_packed16<T>( p, a, q, out, st );
-    } else {
-      launch_f32<T, DECODE>( p, a, q, out, st );
-    }
-  } else {
+  if ( p.waves == 0 ) {
     launch_f32<T, DECODE>( p, a, q, out, st );
+  } else if constexpr ( DECODE ) {
+    launch_decode_tiles<T>( p, a, q, out, st );
+  } else if constexpr ( sizeof( T ) == 2 ) {
+    launch_packed16<T>( p, a, q, out, st );
   }
   GH_LAUNCH_CHECK();
   if ( p.splits > 1 ) {
@@ -1310,7 +1419,7 @@ int attn_pages( const char* op, const void* q, const gh_pages* pages, const uint
     return GH_OK;
   }
   const uint64_t places = reinterpret_cast<uintptr_t>( pages->pool ) | pages->page_stride | reinterpret_cast<uintptr_t>( q ) | reinterpret_cast<uintptr_t>( xb );
-  const Plan p = plan_call( DECODE, batch, rows, max_keys, s, takes16( s, dt ) && places % 16 == 0 && pages->page_tokens >= 16 );
+  const Plan p = plan_call( DECODE, batch, rows, max_keys, s, dt, takes_tiles( s, dt, DECODE ) && places % 16 == 0 && pages->page_tokens >= 16 );
   GH_REQUIRE( p.bytes == 0 || ( workspace != nullptr && reinterpret_cast<uintptr_t>( workspace ) % 16 == 0 ), "%s: a 16-byte aligned workspace is needed", op );
   if ( p.bytes > workspace_bytes ) {
     return fail( GH_ERR_WORKSPACE, "%s: workspace of %llu bytes, %llu are needed", op, (unsigned long long)workspace_bytes, (unsigned long long)p.bytes );
