@@ -69,6 +69,20 @@ __device__ __forceinline__ bool block_of( const Call& a, uint32_t number, uint32
   }
 }
 
+// Block number and kv head of a work-group of packed prompts.  Work-groups go to the 8 XCDs in turn and each has an L2 of its own: where the heads are a multiple
+// of 8 a head's blocks go to one of them, which then fetches its rows once.
+__device__ __forceinline__ void number_and_head( const Call& a, uint32_t* number, uint32_t* h )
+{
+  if ( a.n_kv_heads % 8 == 0 ) {
+    const uint32_t slot = blockIdx.x >> 3, groups = a.n_kv_heads / 8;
+    *number = slot / groups;
+    *h = slot % groups * 8 + ( blockIdx.x & 7 );
+  } else {
+    *number = blockIdx.x / a.n_kv_heads;
+    *h = blockIdx.x % a.n_kv_heads;
+  }
+}
+
 // keys that token t of a block's sequence attends
 __device__ __forceinline__ uint32_t visible( const Call& a, const Block& b, uint32_t t ) { return min( b.start + t + 1, a.max_keys ); }
 
@@ -857,14 +871,7 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
 
   const uint32_t wave = __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 ), lane = threadIdx.x & 63, r = lane & 31, g2 = lane >> 5;
   uint32_t number, h;
-  if ( a.n_kv_heads % 8 == 0 ) {
-    const uint32_t slot = blockIdx.x >> 3, groups = a.n_kv_heads / 8;
-    number = slot / groups;
-    h = slot % groups * 8 + ( blockIdx.x & 7 );
-  } else {
-    number = blockIdx.x / a.n_kv_heads;
-    h = blockIdx.x % a.n_kv_heads;
-  }
+  number_and_head( a, &number, &h );
   Block b;
   if ( !block_of<false, 128>( a, number, h, blockIdx.y, &b ) ) {
     return;
@@ -1144,6 +1151,200 @@ __global__ __launch_bounds__( 256, 2 ) void attn_pages_packed_kernel( const E* _
 }
 
 // =================================================================================================
+// packed prompts in fp32, heads of up to CH chunks of 16 bytes: 64 columns a work-group, 16 a wave
+//
+// Bound by the fp32 matrix instruction (16 x 16, 4 deep) where sequences are long.  Stages of 1024 / CH keys, two of them in LDS: K and V rows go there straight from
+// memory, the next stage's while one is computed, one barrier a stage; rows behind the last key and chunks behind a smaller head arrive as zeros.
+//   S^T = K Q^T     a 16-byte chunk of a key is four steps of the instruction; the scores of a lane: keys 4 g + i of column c
+//   O^T += V^T P^T  the weights are the second operand as they lie, V is read value by value: dim c of a block, of keys 4 g + i
+// Chunks are swizzled by the row so that both reads touch every bank once.
+// =================================================================================================
+template<int CH>
+__device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, float* __restrict__ out, const Call& a )
+{
+  constexpr uint32_t KEYS = 1024 / CH, TILES = KEYS / 16, RPI = 64 / CH, KK = CH / 4, NB = CH / 4;
+  constexpr uint32_t LOADS = 4; // of a wave for a stage's K, and for its V: 4 RPI rows
+  __shared__ mfma_f32x4 s_k0[1024], s_k1[1024], s_v0[1024], s_v1[1024];
+
+  const uint32_t wave = __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 ), lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
+  uint32_t number, h;
+  number_and_head( a, &number, &h );
+  Block b;
+  if ( !block_of<false, 64>( a, number, h, blockIdx.y, &b ) ) {
+    return;
+  }
+  const uint32_t n_heads = a.n_kv_heads * a.gqa, n_cols = b.tokens * a.gqa;
+  const uint32_t k_begin = b.split * a.chunk, k_most = k_begin + a.chunk;
+  auto end_of = [&]( uint32_t token ) { return min( visible( a, b, token ), k_most ); }; // keys a token attends of this split: [k_begin, end)
+  const uint32_t wg_end = __builtin_amdgcn_readfirstlane( end_of( ( min( n_cols, b.col0 + 64 ) - 1 ) / a.gqa ) );
+  if ( wg_end <= k_begin ) {
+    return;
+  }
+  const uint32_t first_col = b.col0 + 16 * wave;
+  const bool wave_ok = first_col < n_cols; // a wave without columns still fetches its share of every stage
+  const uint32_t t_end = __builtin_amdgcn_readfirstlane( wave_ok ? end_of( ( min( n_cols, first_col + 16 ) - 1 ) / a.gqa ) : 0 ); // of some column of the wave
+  const uint32_t t_all = __builtin_amdgcn_readfirstlane( wave_ok ? end_of( first_col / a.gqa ) : 0 );                               // of every column
+  const uint32_t col = first_col + c;
+  const bool ok = col < n_cols;
+  const uint32_t token = ok ? col / a.gqa : 0, head = h * a.gqa + ( ok ? col % a.gqa : 0 );
+  const uint32_t my_end = ok ? end_of( token ) : 0;
+  const uint64_t place = (uint64_t)( b.row0 + token ) * n_heads + head;
+
+  mfma_f32x4 qb[KK];
+#pragma unroll
+  for ( uint32_t kk = 0; kk < KK; kk++ ) {
+    const uint32_t d = 4 * ( 4 * kk + g4 );
+    qb[kk] = ok && d < a.size ? *reinterpret_cast<const mfma_f32x4*>( q + place * a.size + d ) : mfma_f32x4 {};
+  }
+  mfma_f32x4 acc[NB]; // element i of acc[n]: dim 16 n + 4 g4 + i of column c
+#pragma unroll
+  for ( uint32_t n = 0; n < NB; n++ ) {
+    acc[n] = mfma_f32x4 {};
+  }
+  float m = -INFINITY, l = 0.0f; // l: of this lane's keys
+
+  // a lane's place in the rows of a load: the wave's loads are rows 4 RPI wave + RPI t + lane / CH of a stage, which lie in one page
+  const uint32_t ld_row = lane / CH, ld_slot = lane % CH, chunks = a.size / 4, run = 4 * RPI * wave & 15; // run: the wave's first row within its 16
+  const uint32_t k_off = h * a.size * 4, v_off = ( a.n_kv_heads + h ) * a.size * 4;
+  uint32_t k_at[LOADS], v_at[LOADS];
+#pragma unroll
+  for ( uint32_t t = 0; t < LOADS; t++ ) {
+    const uint32_t row = run + RPI * t + ld_row, kc = ld_slot ^ ( row & 15 ), vc = ld_slot ^ ( row & 12 );
+    k_at[t] = kc < chunks ? row * a.pages.row_bytes + k_off + 16 * kc : 0x80000000u;
+    v_at[t] = vc < chunks ? row * a.pages.row_bytes + v_off + 16 * vc : 0x80000000u;
+  }
+  typedef const uint32_t __attribute__( ( address_space( 4 ) ) ) * scalar_ptr;
+  const scalar_ptr table = (scalar_ptr)( reinterpret_cast<uintptr_t>( a.pages.table + (uint64_t)b.seq * a.pages.table_stride ) );
+  const uint32_t first_row = 4 * RPI * wave - run; // of the wave's 16 rows within a stage
+  auto look_up = [&]( uint32_t stage ) __attribute__( ( always_inline ) ) { return table[min( k_begin + KEYS * stage + first_row, wg_end - 1 ) >> a.pages.shift]; };
+  auto fetch = [&]( uint32_t stage, uint32_t id, mfma_f32x4* kt, mfma_f32x4* vt ) __attribute__( ( always_inline ) ) {
+    const uint32_t key = k_begin + KEYS * stage + first_row;
+    const char* base = a.pages.pool + min( id, a.pages.last ) * a.pages.stride + (uint64_t)( key & ( ( 1u << a.pages.shift ) - 1 ) ) * a.pages.row_bytes;
+    const uint32_t rows = key < wg_end ? min( wg_end - key, 16u ) : 0u;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc( const_cast<char*>( base ), 0, (int)( rows * a.pages.row_bytes ), 0x00020000 );
+#pragma unroll
+    for ( uint32_t t = 0; t < LOADS; t++ ) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds( rsrc, (lds_ptr)( kt + ( 4 * RPI * wave + RPI * t ) * CH ), 16, k_at[t], 0, 0, 0 );
+    }
+#pragma unroll
+    for ( uint32_t t = 0; t < LOADS; t++ ) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds( rsrc, (lds_ptr)( vt + ( 4 * RPI * wave + RPI * t ) * CH ), 16, v_at[t], 0, 0, 0 );
+    }
+  };
+
+  const uint32_t n_stages = ( wg_end - k_begin + KEYS - 1 ) / KEYS;
+  fetch( 0, look_up( 0 ), s_k0, s_v0 );
+  uint32_t id = look_up( 1 ); // of the stage behind the one that is computed
+  auto stage = [&]( uint32_t i, const mfma_f32x4* kt, const mfma_f32x4* vt, mfma_f32x4* k_nxt, mfma_f32x4* v_nxt ) __attribute__( ( always_inline ) ) {
+    const uint32_t t0 = k_begin + KEYS * i;
+    __builtin_amdgcn_s_waitcnt( 0x0F70 ); // vmcnt(0): what this wave asked for has landed, behind the barrier what all did, and all are done with the stage before
+    __syncthreads();
+    if ( i + 1 < n_stages ) {
+      fetch( i + 1, id, k_nxt, v_nxt );
+      id = look_up( i + 2 );
+    }
+    if ( t0 >= t_end ) {
+      return; // the whole wave
+    }
+    mfma_f32x4 st[TILES];
+#pragma unroll
+    for ( uint32_t u = 0; u < TILES; u++ ) {
+      st[u] = mfma_f32x4 {};
+#pragma unroll
+      for ( uint32_t kk = 0; kk < KK; kk++ ) {
+        const mfma_f32x4 k = kt[( 16 * u + c ) * CH + ( ( 4 * kk + g4 ) ^ c )];
+#pragma unroll
+        for ( int e = 0; e < 4; e++ ) {
+          st[u] = __builtin_amdgcn_mfma_f32_16x16x4f32( k[e], qb[kk][e], st[u], 0, 0, 0 );
+        }
+      }
+    }
+    if ( __builtin_amdgcn_readfirstlane( t0 + KEYS > t_all ) ) { // keys that some column does not see
+#pragma unroll
+      for ( uint32_t e = 0; e < 4 * TILES; e++ ) {
+        st[e >> 2][e & 3] = t0 + 16 * ( e >> 2 ) + 4 * g4 + ( e & 3 ) < my_end ? st[e >> 2][e & 3] : -INFINITY;
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for ( uint32_t u = 0; u < TILES; u++ ) {
+      mx = fmaxf( mx, fmaxf( fmaxf( st[u][0], st[u][1] ), fmaxf( st[u][2], st[u][3] ) ) );
+    }
+    mx = column_max( mx ) * a.scale_log2e;
+    if ( __builtin_amdgcn_ballot_w64( mx > m + LAZY ) != 0 ) {
+      const float m_new = fmaxf( m, mx ), alpha = m_new == -INFINITY ? 1.0f : fast_exp2( m - m_new );
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for ( uint32_t n = 0; n < NB; n++ ) {
+        acc[n] *= alpha;
+      }
+    }
+    const float ms = m == -INFINITY ? 0.0f : m;
+    float sum[2] = { 0, 0 };
+#pragma unroll
+    for ( uint32_t e = 0; e < 4 * TILES; e++ ) {
+      st[e >> 2][e & 3] = fast_exp2( __builtin_fmaf( st[e >> 2][e & 3], a.scale_log2e, -ms ) );
+      sum[e & 1] += st[e >> 2][e & 3];
+    }
+    l += sum[0] + sum[1];
+    const float* v = reinterpret_cast<const float*>( vt );
+#pragma unroll
+    for ( uint32_t u = 0; u < TILES; u++ ) {
+#pragma unroll
+      for ( uint32_t i4 = 0; i4 < 4; i4++ ) {
+#pragma unroll
+        for ( uint32_t n = 0; n < NB; n++ ) {
+          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32( v[( 16 * u + 4 * g4 + i4 ) * CH * 4 + ( ( 4 * n + ( c >> 2 ) ) ^ ( 4 * g4 ) ) * 4 + ( c & 3 )], st[u][i4], acc[n], 0, 0, 0 );
+        }
+      }
+    }
+  };
+  for ( uint32_t i = 0; i < n_stages; i += 2 ) {
+    stage( i, s_k0, s_v0, s_k1, s_v1 );
+    if ( i + 1 < n_stages ) {
+      stage( i + 1, s_k1, s_v1, s_k0, s_v0 );
+    }
+  }
+
+  l = column_sum( l );
+  float probe = l;
+#pragma unroll
+  for ( uint32_t n = 0; n < NB; n++ ) {
+    probe += 0.0f * ( ( acc[n][0] + acc[n][1] ) + ( acc[n][2] + acc[n][3] ) );
+  }
+  const bool mine = ok && k_begin < my_end;
+  uint64_t again = __builtin_amdgcn_ballot_w64( mine && probe != probe ); // columns with a NaN: once more key by key
+  again = ( again | again >> 16 | again >> 32 | again >> 48 ) & 0xffff;
+  if ( mine && !( again >> c & 1 ) ) {
+    const uint64_t slot = place * a.splits + b.split;
+    const float inv = a.splits > 1 ? 1.0f : 1.0f / l;
+    float* to = a.splits > 1 ? a.part_out + slot * a.size : out + place * a.size;
+#pragma unroll
+    for ( uint32_t n = 0; n < NB; n++ ) {
+      const uint32_t d = 16 * n + 4 * g4;
+      if ( d < a.size ) {
+        store4( to + d, acc[n][0] * inv, acc[n][1] * inv, acc[n][2] * inv, acc[n][3] * inv );
+      }
+    }
+    if ( a.splits > 1 && g4 == 0 ) {
+      a.part_ml[slot * 2] = m;
+      a.part_ml[slot * 2 + 1] = l;
+    }
+  }
+  for ( ; again != 0; again &= again - 1 ) {
+    const uint32_t cl = first_col + (uint32_t)__builtin_ctzll( again );
+    walk_column<float>( q, out, a, b, cl, k_begin, end_of( cl / a.gqa ) );
+  }
+}
+
+template<int CH>
+__global__ __launch_bounds__( 256, 2 ) void attn_pages_packed_f32_kernel( const float* __restrict__ q, float* __restrict__ out, Call a )
+{
+  packed_run_f32<CH>( q, out, a );
+}
+
+// =================================================================================================
 // splits of a row added up: NW waves of a work-group take a (query row, head), every NW-th split each, eight of them asked for at once
 // =================================================================================================
 template<typename T, bool DECODE, int NW>
@@ -1244,11 +1445,8 @@ struct Plan
   uint64_t bytes;
 };
 
-// The 16-bit kernels take heads made of 16-byte chunks, runs of 16 keys in one page, and everything aligned to 16 bytes.
-bool takes_tiles( const gh_shape* s, gh_dtype dt, bool decode )
-{
-  return dt == GH_F32 ? decode && s->head_size % 4 == 0 && s->head_size <= 128 : s->head_size % 8 == 0 && s->head_size <= 128;
-}
+// The kernels that stream to LDS take heads made of 16-byte chunks, runs of 16 keys in one page, and everything aligned to 16 bytes.
+bool takes_tiles( const gh_shape* s, gh_dtype dt ) { return s->head_size * dtype_size( dt ) % 16 == 0 && s->head_size <= 128; }
 
 constexpr uint64_t MOST_PARTS = 65536; // of (query row, head, split) that leave partial results
 
@@ -1256,7 +1454,7 @@ constexpr uint64_t MOST_PARTS = 65536; // of (query row, head, split) that leave
 Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, const gh_shape* s, gh_dtype dt, bool tiles )
 {
   Plan p {};
-  const uint32_t cols = decode ? 16 : tiles ? 128 : 64;
+  const uint32_t cols = decode ? 16 : tiles && dt != GH_F32 ? 128 : 64;
   p.n_blocks = decode ? ( s->gqa_size + cols - 1 ) / cols : 0;
   const uint64_t blocks = decode ? batch * p.n_blocks : std::min<uint64_t>( ( rows * s->gqa_size + cols - 1 ) / cols + batch, rows * s->gqa_size );
   p.blocks = (uint32_t)blocks;
@@ -1294,7 +1492,7 @@ Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, c
     p.bytes = p.splits == 1 ? 0 : rows * s->n_heads * p.splits * ( s->head_size + 2 ) * sizeof( float );
     return p;
   }
-  // as many splits as bring the launch to four work-groups a CU (two of the 16-bit kernel), of at least 256 keys
+  // as many splits as bring the launch to four work-groups a CU (two of the streaming kernels), of at least 256 keys
   const uint64_t groups = blocks * s->n_kv_heads, wanted = ( tiles ? 2ull : 4ull ) * (uint64_t)cu_count();
   const uint64_t splits = std::max<uint64_t>( 1, std::min( { wanted / groups, (uint64_t)( max_keys + 255 ) / 256, MOST_PARTS / ( rows * s->n_heads ) } ) );
   p.waves = tiles ? 4 : 0;
@@ -1361,10 +1559,16 @@ void launch_decode_tiles( const Plan& p, const Call& a, const void* q, void* out
 }
 
 template<typename E>
-void launch_packed16( const Plan& p, const Call& a, const void* q, void* out, hipStream_t st )
+void launch_packed_tiles( const Plan& p, const Call& a, const void* q, void* out, hipStream_t st )
 {
   const dim3 grid( p.blocks * a.n_kv_heads, p.splits );
-  if ( a.size <= 64 ) {
+  if constexpr ( sizeof( E ) == 4 ) {
+    if ( a.size <= 64 ) {
+      attn_pages_packed_f32_kernel<16><<<grid, 256, 0, st>>>( static_cast<const float*>( q ), static_cast<float*>( out ), a );
+    } else {
+      attn_pages_packed_f32_kernel<32><<<grid, 256, 0, st>>>( static_cast<const float*>( q ), static_cast<float*>( out ), a );
+    }
+  } else if ( a.size <= 64 ) {
     attn_pages_packed_kernel<E, 8><<<grid, 256, 0, st>>>( static_cast<const E*>( q ), static_cast<E*>( out ), a );
   } else {
     attn_pages_packed_kernel<E, 16><<<grid, 256, 0, st>>>( static_cast<const E*>( q ), static_cast<E*>( out ), a );
@@ -1378,8 +1582,8 @@ int launch( const Plan& p, const Call& a, const void* q, void* out, uint64_t row
     launch_f32<T, DECODE>( p, a, q, out, st );
   } else if constexpr ( DECODE ) {
     launch_decode_tiles<T>( p, a, q, out, st );
-  } else if constexpr ( sizeof( T ) == 2 ) {
-    launch_packed16<T>( p, a, q, out, st );
+  } else {
+    launch_packed_tiles<T>( p, a, q, out, st );
   }
   GH_LAUNCH_CHECK();
   if ( p.splits > 1 ) {
@@ -1419,7 +1623,7 @@ int attn_pages( const char* op, const void* q, const gh_pages* pages, const uint
     return GH_OK;
   }
   const uint64_t places = reinterpret_cast<uintptr_t>( pages->pool ) | pages->page_stride | reinterpret_cast<uintptr_t>( q ) | reinterpret_cast<uintptr_t>( xb );
-  const Plan p = plan_call( DECODE, batch, rows, max_keys, s, dt, takes_tiles( s, dt, DECODE ) && places % 16 == 0 && pages->page_tokens >= 16 );
+  const Plan p = plan_call( DECODE, batch, rows, max_keys, s, dt, takes_tiles( s, dt ) && places % 16 == 0 && pages->page_tokens >= 16 );
   GH_REQUIRE( p.bytes == 0 || ( workspace != nullptr && reinterpret_cast<uintptr_t>( workspace ) % 16 == 0 ), "%s: a 16-byte aligned workspace is needed", op );
   if ( p.bytes > workspace_bytes ) {
     return fail( GH_ERR_WORKSPACE, "%s: workspace of %llu bytes, %llu are needed", op, (unsigned long long)workspace_bytes, (unsigned long long)p.bytes );
