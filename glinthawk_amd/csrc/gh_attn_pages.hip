@@ -1151,32 +1151,34 @@ __global__ __launch_bounds__( 256, 2 ) void attn_pages_packed_kernel( const E* _
 }
 
 // =================================================================================================
-// packed prompts in fp32, heads of up to CH chunks of 16 bytes: 64 columns a work-group, 16 a wave
+// packed prompts in fp32, heads of up to CH chunks of 16 bytes: 16 CG columns a work-group of two times CG waves, 16 a wave
 //
 // Bound by the fp32 matrix instruction (16 x 16, 4 deep) where sequences are long.  Stages of 1024 / CH keys, two of them in LDS: K and V rows go there straight from
 // memory, the next stage's while one is computed, one barrier a stage; rows behind the last key and chunks behind a smaller head arrive as zeros.
+// The first CG waves take the first half of every stage's keys, the others the second half for the same columns, and are joined through LDS at the end: the longest
+// block of a launch is what a launch of few waits for.
 //   S^T = K Q^T     a 16-byte chunk of a key is four steps of the instruction; the scores of a lane: keys 4 g + i of column c
 //   O^T += V^T P^T  the weights are the second operand as they lie, V is read value by value: dim c of a block, of keys 4 g + i
 // Chunks are swizzled by the row so that both reads touch every bank once.
 // =================================================================================================
-template<int CH>
+template<int CH, int CG>
 __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, float* __restrict__ out, const Call& a )
 {
-  constexpr uint32_t KEYS = 1024 / CH, TILES = KEYS / 16, RPI = 64 / CH, KK = CH / 4, NB = CH / 4;
-  constexpr uint32_t LOADS = 4; // of a wave for a stage's K, and for its V: 4 RPI rows
+  constexpr uint32_t KEYS = 1024 / CH, TILES = KEYS / 32, RPI = 64 / CH, KK = CH / 4, NB = CH / 4;
+  constexpr uint32_t LOADS = 8 / CG; // of a wave for a stage's K, and for its V
   __shared__ mfma_f32x4 s_k0[1024], s_k1[1024], s_v0[1024], s_v1[1024];
 
-  const uint32_t wave = __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 ), lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
+  const uint32_t loader = __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 ), wave = loader % CG, part = loader / CG, lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
   uint32_t number, h;
   number_and_head( a, &number, &h );
   Block b;
-  if ( !block_of<false, 64>( a, number, h, blockIdx.y, &b ) ) {
+  if ( !block_of<false, 16 * CG>( a, number, h, blockIdx.y, &b ) ) {
     return;
   }
   const uint32_t n_heads = a.n_kv_heads * a.gqa, n_cols = b.tokens * a.gqa;
   const uint32_t k_begin = b.split * a.chunk, k_most = k_begin + a.chunk;
   auto end_of = [&]( uint32_t token ) { return min( visible( a, b, token ), k_most ); }; // keys a token attends of this split: [k_begin, end)
-  const uint32_t wg_end = __builtin_amdgcn_readfirstlane( end_of( ( min( n_cols, b.col0 + 64 ) - 1 ) / a.gqa ) );
+  const uint32_t wg_end = __builtin_amdgcn_readfirstlane( end_of( ( min( n_cols, b.col0 + 16 * CG ) - 1 ) / a.gqa ) );
   if ( wg_end <= k_begin ) {
     return;
   }
@@ -1203,8 +1205,8 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
   }
   float m = -INFINITY, l = 0.0f; // l: of this lane's keys
 
-  // a lane's place in the rows of a load: the wave's loads are rows 4 RPI wave + RPI t + lane / CH of a stage, which lie in one page
-  const uint32_t ld_row = lane / CH, ld_slot = lane % CH, chunks = a.size / 4, run = 4 * RPI * wave & 15; // run: the wave's first row within its 16
+  // a lane's place in the rows of a load: the wave's loads are rows RPI (LOADS loader + t) + lane / CH of a stage, which lie in one page
+  const uint32_t ld_row = lane / CH, ld_slot = lane % CH, chunks = a.size / 4, run = LOADS * RPI * loader & 15; // run: the wave's first row within its 16
   const uint32_t k_off = h * a.size * 4, v_off = ( a.n_kv_heads + h ) * a.size * 4;
   uint32_t k_at[LOADS], v_at[LOADS];
 #pragma unroll
@@ -1215,7 +1217,7 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
   }
   typedef const uint32_t __attribute__( ( address_space( 4 ) ) ) * scalar_ptr;
   const scalar_ptr table = (scalar_ptr)( reinterpret_cast<uintptr_t>( a.pages.table + (uint64_t)b.seq * a.pages.table_stride ) );
-  const uint32_t first_row = 4 * RPI * wave - run; // of the wave's 16 rows within a stage
+  const uint32_t first_row = LOADS * RPI * loader - run; // of the wave's 16 rows within a stage
   auto look_up = [&]( uint32_t stage ) __attribute__( ( always_inline ) ) { return table[min( k_begin + KEYS * stage + first_row, wg_end - 1 ) >> a.pages.shift]; };
   auto fetch = [&]( uint32_t stage, uint32_t id, mfma_f32x4* kt, mfma_f32x4* vt ) __attribute__( ( always_inline ) ) {
     const uint32_t key = k_begin + KEYS * stage + first_row;
@@ -1224,11 +1226,11 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc( const_cast<char*>( base ), 0, (int)( rows * a.pages.row_bytes ), 0x00020000 );
 #pragma unroll
     for ( uint32_t t = 0; t < LOADS; t++ ) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds( rsrc, (lds_ptr)( kt + ( 4 * RPI * wave + RPI * t ) * CH ), 16, k_at[t], 0, 0, 0 );
+      __builtin_amdgcn_raw_ptr_buffer_load_lds( rsrc, (lds_ptr)( kt + ( LOADS * RPI * loader + RPI * t ) * CH ), 16, k_at[t], 0, 0, 0 );
     }
 #pragma unroll
     for ( uint32_t t = 0; t < LOADS; t++ ) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds( rsrc, (lds_ptr)( vt + ( 4 * RPI * wave + RPI * t ) * CH ), 16, v_at[t], 0, 0, 0 );
+      __builtin_amdgcn_raw_ptr_buffer_load_lds( rsrc, (lds_ptr)( vt + ( LOADS * RPI * loader + RPI * t ) * CH ), 16, v_at[t], 0, 0, 0 );
     }
   };
 
@@ -1236,7 +1238,7 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
   fetch( 0, look_up( 0 ), s_k0, s_v0 );
   uint32_t id = look_up( 1 ); // of the stage behind the one that is computed
   auto stage = [&]( uint32_t i, const mfma_f32x4* kt, const mfma_f32x4* vt, mfma_f32x4* k_nxt, mfma_f32x4* v_nxt ) __attribute__( ( always_inline ) ) {
-    const uint32_t t0 = k_begin + KEYS * i;
+    const uint32_t r0 = 16 * TILES * part, t0 = k_begin + KEYS * i + r0; // the wave's first row of the stage, its key
     __builtin_amdgcn_s_waitcnt( 0x0F70 ); // vmcnt(0): what this wave asked for has landed, behind the barrier what all did, and all are done with the stage before
     __syncthreads();
     if ( i + 1 < n_stages ) {
@@ -1252,14 +1254,14 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
       st[u] = mfma_f32x4 {};
 #pragma unroll
       for ( uint32_t kk = 0; kk < KK; kk++ ) {
-        const mfma_f32x4 k = kt[( 16 * u + c ) * CH + ( ( 4 * kk + g4 ) ^ c )];
+        const mfma_f32x4 k = kt[( r0 + 16 * u + c ) * CH + ( ( 4 * kk + g4 ) ^ c )];
 #pragma unroll
         for ( int e = 0; e < 4; e++ ) {
           st[u] = __builtin_amdgcn_mfma_f32_16x16x4f32( k[e], qb[kk][e], st[u], 0, 0, 0 );
         }
       }
     }
-    if ( __builtin_amdgcn_readfirstlane( t0 + KEYS > t_all ) ) { // keys that some column does not see
+    if ( __builtin_amdgcn_readfirstlane( t0 + 16 * TILES > t_all ) ) { // keys that some column does not see
 #pragma unroll
       for ( uint32_t e = 0; e < 4 * TILES; e++ ) {
         st[e >> 2][e & 3] = t0 + 16 * ( e >> 2 ) + 4 * g4 + ( e & 3 ) < my_end ? st[e >> 2][e & 3] : -INFINITY;
@@ -1295,7 +1297,7 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
       for ( uint32_t i4 = 0; i4 < 4; i4++ ) {
 #pragma unroll
         for ( uint32_t n = 0; n < NB; n++ ) {
-          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32( v[( 16 * u + 4 * g4 + i4 ) * CH * 4 + ( ( 4 * n + ( c >> 2 ) ) ^ ( 4 * g4 ) ) * 4 + ( c & 3 )], st[u][i4], acc[n], 0, 0, 0 );
+          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32( v[( r0 + 16 * u + 4 * g4 + i4 ) * CH * 4 + ( ( 4 * n + ( c >> 2 ) ) ^ ( 4 * g4 ) ) * 4 + ( c & 3 )], st[u][i4], acc[n], 0, 0, 0 );
         }
       }
     }
@@ -1308,6 +1310,39 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
   }
 
   l = column_sum( l );
+  // the second half's parts, lane for lane as they lie in the registers
+  constexpr uint32_t PART = 64 * ( 4 * NB + 2 );
+  static_assert( PART * 4 <= sizeof( s_k0 ), "a wave's part fits one of the arrays" );
+  float* parts = reinterpret_cast<float*>( wave == 0 ? s_k0 : wave == 1 ? s_k1 : wave == 2 ? s_v0 : s_v1 );
+  __syncthreads();
+  if ( part == 1 ) {
+    parts[lane] = m;
+    parts[64 + lane] = l;
+#pragma unroll
+    for ( uint32_t n = 0; n < NB; n++ ) {
+#pragma unroll
+      for ( int i = 0; i < 4; i++ ) {
+        parts[( 2 + 4 * n + i ) * 64 + lane] = acc[n][i];
+      }
+    }
+  }
+  __syncthreads();
+  if ( part == 1 ) {
+    return;
+  }
+  {
+    const float other = parts[lane], mm = fmaxf( m, other ), mm_safe = mm == -INFINITY ? 0.0f : mm;
+    const float w0 = fast_exp2( m - mm_safe ), w1 = fast_exp2( other - mm_safe );
+    m = mm;
+    l = l * w0 + parts[64 + lane] * w1;
+#pragma unroll
+    for ( uint32_t n = 0; n < NB; n++ ) {
+#pragma unroll
+      for ( int i = 0; i < 4; i++ ) {
+        acc[n][i] = __builtin_fmaf( parts[( 2 + 4 * n + i ) * 64 + lane], w1, acc[n][i] * w0 );
+      }
+    }
+  }
   float probe = l;
 #pragma unroll
   for ( uint32_t n = 0; n < NB; n++ ) {
@@ -1338,10 +1373,10 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
   }
 }
 
-template<int CH>
-__global__ __launch_bounds__( 256, 2 ) void attn_pages_packed_f32_kernel( const float* __restrict__ q, float* __restrict__ out, Call a )
+template<int CH, int CG>
+__global__ __launch_bounds__( 128 * CG, CG ) void attn_pages_packed_f32_kernel( const float* __restrict__ q, float* __restrict__ out, Call a )
 {
-  packed_run_f32<CH>( q, out, a );
+  packed_run_f32<CH, CG>( q, out, a );
 }
 
 // =================================================================================================
@@ -1454,9 +1489,15 @@ constexpr uint64_t MOST_PARTS = 65536; // of (query row, head, split) that leave
 Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, const gh_shape* s, gh_dtype dt, bool tiles )
 {
   Plan p {};
-  const uint32_t cols = decode ? 16 : tiles && dt != GH_F32 ? 128 : 64;
+  uint32_t cols = decode ? 16 : tiles && dt != GH_F32 ? 128 : 64;
+  auto blocks_of = [&] { return std::min<uint64_t>( ( rows * s->gqa_size + cols - 1 ) / cols + batch, rows * s->gqa_size ); };
+  // fp32: half as many columns a work-group while there are fewer than two and a half a CU, since a launch of few lasts as long as its longest (5 prompts of 100 to 900 tokens, 12
+  // heads of 64: 51 us with 64 columns, 40 with 32; 4 of 300, 32 heads of 128: 46 and 49; 16 of 1000, 12 heads of 64: 254 and 294)
+  if ( !decode && tiles && dt == GH_F32 && blocks_of() * s->n_kv_heads * 2 < 5ull * (uint64_t)cu_count() ) {
+    cols = 32;
+  }
   p.n_blocks = decode ? ( s->gqa_size + cols - 1 ) / cols : 0;
-  const uint64_t blocks = decode ? batch * p.n_blocks : std::min<uint64_t>( ( rows * s->gqa_size + cols - 1 ) / cols + batch, rows * s->gqa_size );
+  const uint64_t blocks = decode ? batch * p.n_blocks : blocks_of();
   p.blocks = (uint32_t)blocks;
   if ( decode && tiles ) {
     // Microseconds as measured on MI355X.  A stage of 16 KB takes a wave on its own 0.75, the four waves of a work-group 1.5, and 2.4 where the waves that fit
@@ -1492,10 +1533,21 @@ Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, c
     p.bytes = p.splits == 1 ? 0 : rows * s->n_heads * p.splits * ( s->head_size + 2 ) * sizeof( float );
     return p;
   }
-  // as many splits as bring the launch to four work-groups a CU (two of the streaming kernels), of at least 256 keys
-  const uint64_t groups = blocks * s->n_kv_heads, wanted = ( tiles ? 2ull : 4ull ) * (uint64_t)cu_count();
-  const uint64_t splits = std::max<uint64_t>( 1, std::min( { wanted / groups, (uint64_t)( max_keys + 255 ) / 256, MOST_PARTS / ( rows * s->n_heads ) } ) );
-  p.waves = tiles ? 4 : 0;
+  // Few rows of many keys: as many splits as cost least.  A stage of 64 keys takes a work-group 1.1 us (2.6 in fp32); a split adds a launch (5) and 8 bytes an element that go
+  // out and come back at 2 TB/s.  us, f16, 8 kv heads of 8 queries: 64 tokens behind 4000 keys, unsplit 76, in 6 33, in 16 35 | 16 behind 30000: 502, in 16 50, in 32 45 |
+  // 512 tokens: 20, in 2 48.  fp32, 12 heads of 64: 64 tokens behind 2000 keys: 86, in 16 20, in 32 23.
+  const uint64_t groups = blocks * s->n_kv_heads;
+  uint64_t splits = 1;
+  double best = 0;
+  for ( uint64_t n = 1; n <= 256 && ( n == 1 || ( rows * s->n_heads * n <= MOST_PARTS && ( n - 1 ) * 64 < max_keys ) ); n += ( n + 1 ) / 2 ) {
+    const double stages = (double)( ( ( max_keys + n - 1 ) / n + 63 ) / 64 ), load = (double)( groups * n ) / ( 2.0 * cu_count() );
+    const double us = stages * ( dt == GH_F32 ? 2.6 : 1.1 ) * std::max( 1.0, load ) + ( n > 1 ? 5.0 + (double)( rows * s->n_heads * n ) * s->head_size * 8 / 2e6 : 0.0 );
+    if ( n == 1 || us < best ) {
+      best = us;
+      splits = n;
+    }
+  }
+  p.waves = !tiles ? 0 : dt == GH_F32 ? cols / 8 : 4;
   p.chunk = (uint32_t)( ( ( max_keys + splits - 1 ) / splits + 63 ) / 64 * 64 );
   p.splits = ( max_keys + p.chunk - 1 ) / p.chunk;
   p.bytes = p.splits == 1 ? 0 : rows * s->n_heads * p.splits * ( s->head_size + 2 ) * sizeof( float );
@@ -1563,10 +1615,12 @@ void launch_packed_tiles( const Plan& p, const Call& a, const void* q, void* out
 {
   const dim3 grid( p.blocks * a.n_kv_heads, p.splits );
   if constexpr ( sizeof( E ) == 4 ) {
+    const float* tq = static_cast<const float*>( q );
+    float* to = static_cast<float*>( out );
     if ( a.size <= 64 ) {
-      attn_pages_packed_f32_kernel<16><<<grid, 256, 0, st>>>( static_cast<const float*>( q ), static_cast<float*>( out ), a );
+      p.waves == 8 ? attn_pages_packed_f32_kernel<16, 4><<<grid, 512, 0, st>>>( tq, to, a ) : attn_pages_packed_f32_kernel<16, 2><<<grid, 256, 0, st>>>( tq, to, a );
     } else {
-      attn_pages_packed_f32_kernel<32><<<grid, 256, 0, st>>>( static_cast<const float*>( q ), static_cast<float*>( out ), a );
+      p.waves == 8 ? attn_pages_packed_f32_kernel<32, 4><<<grid, 512, 0, st>>>( tq, to, a ) : attn_pages_packed_f32_kernel<32, 2><<<grid, 256, 0, st>>>( tq, to, a );
     }
   } else if ( a.size <= 64 ) {
     attn_pages_packed_kernel<E, 8><<<grid, 256, 0, st>>>( static_cast<const E*>( q ), static_cast<E*>( out ), a );

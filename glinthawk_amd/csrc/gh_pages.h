@@ -66,13 +66,24 @@ struct Packed
   }
 };
 
+// sum or maximum over the wave, in every lane: rows of 16 lanes by DPP, the four rows by lane reads
+template<typename F>
+__device__ __forceinline__ uint32_t wave_all( uint32_t v, F f )
+{
+  v = f( v, (uint32_t)__builtin_amdgcn_update_dpp( 0, (int)v, 0xB1, 0xF, 0xF, true ) );
+  v = f( v, (uint32_t)__builtin_amdgcn_update_dpp( 0, (int)v, 0x4E, 0xF, 0xF, true ) );
+  v = f( v, (uint32_t)__builtin_amdgcn_update_dpp( 0, (int)v, 0x141, 0xF, 0xF, true ) );
+  v = f( v, (uint32_t)__builtin_amdgcn_update_dpp( 0, (int)v, 0x140, 0xF, 0xF, true ) );
+  return f( f( (uint32_t)__builtin_amdgcn_readlane( (int)v, 0 ), (uint32_t)__builtin_amdgcn_readlane( (int)v, 16 ) ),
+            f( (uint32_t)__builtin_amdgcn_readlane( (int)v, 32 ), (uint32_t)__builtin_amdgcn_readlane( (int)v, 48 ) ) );
+}
 __device__ __forceinline__ uint32_t wave_sum_u32( uint32_t v )
 {
-#pragma unroll
-  for ( int off = 32; off > 0; off >>= 1 ) {
-    v += __shfl_xor( v, off, WAVE );
-  }
-  return v;
+  return wave_all( v, []( uint32_t a, uint32_t b ) { return a + b; } );
+}
+__device__ __forceinline__ uint32_t wave_max_u32( uint32_t v )
+{
+  return wave_all( v, []( uint32_t a, uint32_t b ) { return a > b ? a : b; } );
 }
 
 // Block number -> (sequence, block of the sequence), by a whole wave.  A sequence of n tokens with `gqa` columns each has ceil(n gqa / columns) blocks; blocks
@@ -87,10 +98,7 @@ __device__ __forceinline__ bool packed_block( const Packed& s, uint32_t gqa, uin
   for ( uint32_t i = 64 + lane; i < s.batch; i += 64 ) {
     most = max( most, blocks( i ) );
   }
-#pragma unroll
-  for ( int off = 32; off > 0; off >>= 1 ) {
-    most = max( most, __shfl_xor( most, off, WAVE ) );
-  }
+  most = wave_max_u32( most );
   auto above = [&]( uint32_t level ) { // blocks at `level` and beyond
     uint32_t n = mine > level ? mine - level : 0;
     for ( uint32_t i = 64 + lane; i < s.batch; i += 64 ) {
