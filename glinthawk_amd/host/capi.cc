@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "glint/contextman.hh"
+#include "glint/pages.hh"
 #include "glint/designs.hh"
 #include "glint/kernel.hh"
 #include "glint/loader.hh"
@@ -538,6 +539,76 @@ int glint_book_stands_twice( const uint64_t* memory, uint64_t n )
 }
 
 int glint_book_manager_release( void* m, uint32_t context_id ) { return static_cast<BookManager*>( m )->man.release_context( context_id ) ? 1 : 0; }
+
+// pages of a pool and the contexts that have them (glint/pages.hh).  A call that runs out of memory says that it failed.
+void* glint_pages_new( uint32_t n_pages, uint32_t page_tokens )
+{
+  try {
+    return n_pages == 0 || page_tokens == 0 ? nullptr : new PageBook( n_pages, page_tokens );
+  } catch ( const std::bad_alloc& ) {
+    return nullptr;
+  }
+}
+void glint_pages_delete( void* b ) { delete static_cast<PageBook*>( b ); }
+uint64_t glint_pages_free( void* b ) { return static_cast<PageBook*>( b )->free(); }
+// the number of copies to make (0 or 1, in pair), or -1: not enough pages, nothing changed
+int glint_pages_extend( void* b, uint64_t id, uint64_t tokens, uint32_t pair[2] )
+{
+  try {
+    const auto pairs = static_cast<PageBook*>( b )->extend( id, tokens );
+    if ( !pairs.has_value() ) {
+      return -1;
+    }
+    if ( !pairs->empty() ) {
+      pair[0] = pairs->front().first;
+      pair[1] = pairs->front().second;
+    }
+    return static_cast<int>( pairs->size() );
+  } catch ( const std::bad_alloc& ) {
+    return -1;
+  }
+}
+int glint_pages_fork( void* b, uint64_t parent, uint64_t child )
+{
+  try {
+    return static_cast<PageBook*>( b )->fork( parent, child ) ? 1 : 0;
+  } catch ( const std::bad_alloc& ) {
+    return -1;
+  }
+}
+int glint_pages_release( void* b, uint64_t id ) { return static_cast<PageBook*>( b )->release( id ) ? 1 : 0; }
+// the number of copies to make; up to cap of them in pairs
+int64_t glint_pages_compact( void* b, uint32_t* pairs, uint64_t cap )
+{
+  try {
+    const auto moved = static_cast<PageBook*>( b )->compact();
+    for ( size_t i = 0; i < moved.size() && i < cap; i++ ) {
+      pairs[2 * i] = moved[i].first;
+      pairs[2 * i + 1] = moved[i].second;
+    }
+    return static_cast<int64_t>( moved.size() );
+  } catch ( const std::bad_alloc& ) {
+    return -1;
+  }
+}
+// tokens of a context, -1: not known
+int64_t glint_pages_length( void* b, uint64_t id )
+{
+  const auto context = static_cast<PageBook*>( b )->context( id );
+  return context ? static_cast<int64_t>( context->length ) : -1;
+}
+// the number of a context's pages, up to cap of them in out; -1: not known
+int64_t glint_pages_line( void* b, uint64_t id, uint32_t* out, uint64_t cap )
+{
+  const auto context = static_cast<PageBook*>( b )->context( id );
+  if ( !context ) {
+    return -1;
+  }
+  for ( size_t i = 0; i < context->pages.size() && i < cap; i++ ) {
+    out[i] = context->pages[i];
+  }
+  return static_cast<int64_t>( context->pages.size() );
+}
 
 // paged context over a counting region: hosts `n_hosted` layers of the 70B-4K shape
 void* glint_book_paged_new( uint32_t n_hosted ) { return new PagedBookContext( StageSettings<BookConfig>::slice( 0, n_hosted, 1, 1 ) ); }

@@ -84,6 +84,15 @@ def host_lib() -> C.CDLL:
             "glint_book_manager_get_context": (i32, [vp, u32]),
             "glint_book_manager_release": (C.c_int, [vp, u32]),
             "glint_book_stands_twice": (C.c_int, [vp, u64]),
+            "glint_pages_new": (vp, [u32, u32]),
+            "glint_pages_delete": (None, [vp]),
+            "glint_pages_free": (u64, [vp]),
+            "glint_pages_extend": (C.c_int, [vp, u64, u64, C.POINTER(u32)]),
+            "glint_pages_fork": (C.c_int, [vp, u64, u64]),
+            "glint_pages_release": (C.c_int, [vp, u64]),
+            "glint_pages_compact": (C.c_int64, [vp, C.POINTER(u32), u64]),
+            "glint_pages_length": (C.c_int64, [vp, u64]),
+            "glint_pages_line": (C.c_int64, [vp, u64, C.POINTER(u32), u64]),
             "glint_book_paged_new": (vp, [u32]),
             "glint_book_paged_delete": (None, [vp]),
             "glint_book_paged_prepare": (u64, [vp, u32, u32, C.c_int, C.POINTER(u64)]),
