@@ -440,6 +440,13 @@ def _refuse(pool: torch.Tensor, **wanted) -> None:
     raise ValueError("the page table has fewer contexts than the batch, or the rows of the pool are not the shape's")
 
 
+def _stream_on(device: torch.device) -> int:
+    """The current stream.  By its number straight away: as an object it takes 2.7 us of a call's 8."""
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {device}, which is not the current GPU")
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 @functools.lru_cache(maxsize=None)
 def _shape_ref(shape: Shape):
     return C.byref(shape.c())
@@ -466,7 +473,7 @@ def page_rows(p: GhPages, first: torch.Tensor, start_pos: Optional[torch.Tensor]
         _refuse(p.pool_tensor, first=(first, torch.int32, (batch + 1,)), start_pos=(start_pos, torch.int32, (batch,)))
     rows = torch.empty(n_tokens, dtype=torch.int64, device=p.device)
     pos = torch.empty(n_tokens, dtype=torch.int32, device=p.device)
-    check(lib().gh_page_rows(C.byref(p), first.data_ptr(), _p(start_pos), batch, n_tokens, p.row // 2, _p(rows), _p(pos), p.dt, _stream()), "gh_page_rows")
+    check(lib().gh_page_rows(C.byref(p), first.data_ptr(), _p(start_pos), batch, n_tokens, p.row // 2, _p(rows), _p(pos), p.dt, _stream_on(p.device)), "gh_page_rows")
     return rows, pos
 
 
@@ -486,7 +493,7 @@ def attn_decode_paged(q: torch.Tensor, p: GhPages, lengths: torch.Tensor, xb: to
     if workspace is None:
         workspace = torch.empty(attn_decode_paged_workspace(batch, max_length, shape, q.dtype), dtype=torch.uint8, device=q.device)
     check(lib().gh_attn_decode_paged(q.data_ptr(), C.byref(p), lengths.data_ptr(), xb.data_ptr(), batch, max_length, _shape_ref(shape), p.dt, workspace.data_ptr(),
-                                     workspace.nbytes, _stream()), "gh_attn_decode_paged")
+                                     workspace.nbytes, _stream_on(p.device)), "gh_attn_decode_paged")
 
 
 def attn_packed_workspace(batch: int, n_tokens: int, max_keys: int, shape: Shape, dtype: torch.dtype) -> int:
@@ -507,7 +514,7 @@ def attn_packed(q: torch.Tensor, p: GhPages, first: torch.Tensor, start_pos: Opt
     if workspace is None:
         workspace = torch.empty(attn_packed_workspace(batch, tokens, max_keys, shape, q.dtype), dtype=torch.uint8, device=q.device)
     check(lib().gh_attn_packed(q.data_ptr(), C.byref(p), first.data_ptr(), _p(start_pos), xb.data_ptr(), batch, tokens, max_keys, _shape_ref(shape), p.dt,
-                               workspace.data_ptr(), workspace.nbytes, _stream()), "gh_attn_packed")
+                               workspace.data_ptr(), workspace.nbytes, _stream_on(p.device)), "gh_attn_packed")
 
 
 def copy_pages(pool: torch.Tensor, pairs) -> None:
@@ -521,10 +528,10 @@ def copy_pages(pool: torch.Tensor, pairs) -> None:
     if isinstance(pairs, torch.Tensor):
         if not (pairs.dtype is torch.int32 and pairs.dim() == 2 and pairs.shape[1] == 2 and pairs.is_contiguous() and pairs.device == pool.device):
             _refuse(pool, pairs=(pairs, torch.int32, (pairs.shape[0] if pairs.dim() else 0, 2)))
-        check(lib().gh_copy_pages(*common, pairs.data_ptr(), pairs.shape[0], _stream()), "gh_copy_pages")
+        check(lib().gh_copy_pages(*common, pairs.data_ptr(), pairs.shape[0], _stream_on(pool.device)), "gh_copy_pages")
     else:
         flat = [int(v) for pair in pairs for v in pair]
-        check(lib().gh_copy_pages_host(*common, host_u32_array(flat), len(flat) // 2, _stream()), "gh_copy_pages_host")
+        check(lib().gh_copy_pages_host(*common, host_u32_array(flat), len(flat) // 2, _stream_on(pool.device)), "gh_copy_pages_host")
 
 
 def token_logprobs_workspace(rows: int, vocab: int, n_top: int) -> int:
@@ -545,7 +552,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, n_top: int = 0, w
     ids = torch.empty((rows, n_top), dtype=torch.int32, device=device)
     values = torch.empty((rows, n_top), dtype=torch.float32, device=device)
     check(lib().gh_token_logprobs(given.data_ptr(), entropy.data_ptr(), ids.data_ptr(), values.data_ptr(), logits.data_ptr(), logits.stride(0), tokens.data_ptr(), vocab, rows,
-                                  n_top, _dt(logits), workspace.data_ptr(), workspace.nbytes, _stream()), "gh_token_logprobs")
+                                  n_top, _dt(logits), workspace.data_ptr(), workspace.nbytes, _stream_on(device)), "gh_token_logprobs")
     return given, entropy, ids, values
 
 
