@@ -55,16 +55,16 @@ __device__ __forceinline__ bool block_of( const Call& a, uint32_t number, uint32
     b->start = length - 1;
     return true;
   } else {
-    uint32_t seq, block;
-    if ( !packed_block( a.seqs, a.gqa, COLS, number, &seq, &block ) ) {
+    PackedBlock f;
+    if ( !packed_block( a.seqs, a.gqa, COLS, number, &f ) ) {
       return false;
     }
     // (said to be the same in every lane: what descriptors and branches are made of stays in scalar registers)
-    b->seq = __builtin_amdgcn_readfirstlane( seq );
-    b->col0 = __builtin_amdgcn_readfirstlane( block ) * COLS;
-    b->row0 = __builtin_amdgcn_readfirstlane( a.seqs.begin( b->seq ) );
-    b->tokens = __builtin_amdgcn_readfirstlane( a.seqs.count( b->seq ) );
-    b->start = __builtin_amdgcn_readfirstlane( a.seqs.start ? min( a.seqs.start[b->seq], 0x7fffffffu ) : 0u );
+    b->seq = __builtin_amdgcn_readfirstlane( f.seq );
+    b->col0 = __builtin_amdgcn_readfirstlane( f.block ) * COLS;
+    b->row0 = __builtin_amdgcn_readfirstlane( f.row0 );
+    b->tokens = __builtin_amdgcn_readfirstlane( f.tokens );
+    b->start = __builtin_amdgcn_readfirstlane( f.start );
     return true;
   }
 }
@@ -1397,8 +1397,7 @@ __global__ __launch_bounds__( 256 ) void pages_merge_kernel( T* __restrict__ out
     } else {
       const uint32_t seq = packed_sequence( a.seqs, row );
       if ( seq < a.seqs.batch && row - a.seqs.begin( seq ) < a.seqs.count( seq ) ) {
-        const uint32_t start = a.seqs.start ? min( a.seqs.start[seq], 0x7fffffffu ) : 0u;
-        keys = min( start + ( row - a.seqs.begin( seq ) ) + 1, a.max_keys );
+        keys = min( a.seqs.begin_pos( seq ) + ( row - a.seqs.begin( seq ) ) + 1, a.max_keys );
       }
     }
   }

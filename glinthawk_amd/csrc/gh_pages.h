@@ -64,6 +64,8 @@ struct Packed
     const uint32_t b = begin( i ), e = begin( i + 1 );
     return e > b ? e - b : 0;
   }
+  // position of its first token, so that sums of it and a number of tokens stay below 2^32
+  __device__ __forceinline__ uint32_t begin_pos( uint32_t i ) const { return start ? min( start[i], 0x3fffffffu ) : 0u; }
 };
 
 // sum or maximum over the wave, in every lane: rows of 16 lanes by DPP, the four rows by lane reads
@@ -86,24 +88,42 @@ __device__ __forceinline__ uint32_t wave_max_u32( uint32_t v )
   return wave_all( v, []( uint32_t a, uint32_t b ) { return a > b ? a : b; } );
 }
 
-// Block number -> (sequence, block of the sequence), by a whole wave.  A sequence of n tokens with `gqa` columns each has ceil(n gqa / columns) blocks; blocks
-// are numbered by falling position in their sequence, so that the ones with the most keys come first and a launch does not end on a long one.  The level (position) of
-// a number is found by bisection over how many blocks lie at a level and above, a sum over the sequences.  False: no such block.
-__device__ __forceinline__ bool packed_block( const Packed& s, uint32_t gqa, uint32_t columns, uint32_t number, uint32_t* seq, uint32_t* block )
+// Block number -> (sequence, block of the sequence), by a whole wave.  A sequence of n tokens with `gqa` columns each has ceil(n gqa / columns) blocks.  Blocks are
+// numbered by falling level, which is the block's place in its sequence plus the blocks that the sequence's start position would be, so that the ones with the most
+// keys come first and a launch does not end on a long one.  The level of a number is found by bisection over how many blocks lie at a level and above, a sum over the
+// sequences.  False: no such block.
+// A sequence as packed_block found it
+struct PackedBlock
+{
+  uint32_t seq, block;
+  uint32_t row0, tokens, start; // of the sequence
+};
+__device__ __forceinline__ bool packed_block( const Packed& s, uint32_t gqa, uint32_t columns, uint32_t number, PackedBlock* found )
 {
   const uint32_t lane = threadIdx.x & 63;
-  auto blocks = [&]( uint32_t i ) { return i < s.batch ? (uint32_t)( ( (uint64_t)s.count( i ) * gqa + columns - 1 ) / columns ) : 0u; };
-  const uint32_t mine = blocks( lane ); // those of the first 64 sequences are kept
-  uint32_t most = mine;
+  auto blocks_of = [&]( uint32_t tokens ) { return (uint32_t)( ( (uint64_t)tokens * gqa + columns - 1 ) / columns ); };
+  auto blocks = [&]( uint32_t i ) { return i < s.batch ? blocks_of( s.count( i ) ) : 0u; };
+  auto level_of = [&]( uint32_t start ) { return (uint32_t)min( (uint64_t)start * gqa / columns, (uint64_t)0x3fffffff ); }; // of a sequence's first block
+  auto level0 = [&]( uint32_t i ) { return i < s.batch ? level_of( s.begin_pos( i ) ) : 0u; };
+  // what there is to know of the first 64 sequences is read once, and kept
+  const uint32_t at = min( lane, s.batch - 1 ), my_row0 = s.begin( at ), my_tokens = s.count( at ), my_start = s.begin_pos( at );
+  if ( s.batch == 1 ) {
+    const uint32_t n = blocks_of( my_tokens );
+    *found = { 0, n - 1 - number, my_row0, my_tokens, my_start };
+    return number < n;
+  }
+  const uint32_t mine = lane < s.batch ? blocks_of( my_tokens ) : 0, mine0 = level_of( my_start );
+  uint32_t most = mine == 0 ? 0 : mine0 + mine;
   for ( uint32_t i = 64 + lane; i < s.batch; i += 64 ) {
-    most = max( most, blocks( i ) );
+    const uint32_t n = blocks( i );
+    most = max( most, n == 0 ? 0 : level0( i ) + n );
   }
   most = wave_max_u32( most );
   auto above = [&]( uint32_t level ) { // blocks at `level` and beyond
-    uint32_t n = mine > level ? mine - level : 0;
+    uint32_t n = min( mine, mine0 + mine > level ? mine0 + mine - level : 0u );
     for ( uint32_t i = 64 + lane; i < s.batch; i += 64 ) {
-      const uint32_t b = blocks( i );
-      n += b > level ? b - level : 0;
+      const uint32_t b = blocks( i ), end = level0( i ) + b;
+      n += min( b, end > level ? end - level : 0u );
     }
     return wave_sum_u32( n );
   };
@@ -121,13 +141,24 @@ __device__ __forceinline__ bool packed_block( const Packed& s, uint32_t gqa, uin
   }
   uint32_t rank = number - above( low + 1 ); // among the sequences that have a block at this level
   for ( uint32_t i0 = 0; i0 < s.batch; i0 += 64 ) {
-    const uint64_t have = __builtin_amdgcn_ballot_w64( ( i0 == 0 ? mine : blocks( i0 + lane ) ) > low );
+    const uint32_t first = i0 == 0 ? mine0 : level0( i0 + lane ), n_blocks = i0 == 0 ? mine : blocks( i0 + lane );
+    const uint64_t have = __builtin_amdgcn_ballot_w64( first <= low && low < first + n_blocks );
     const uint32_t n = __popcll( have );
     if ( rank < n ) {
       // the lane whose set bit has `rank` set bits below it
       const uint64_t hit = __builtin_amdgcn_ballot_w64( ( have >> lane & 1 ) && (uint32_t)__popcll( have & ( ( 1ull << lane ) - 1 ) ) == rank );
-      *seq = i0 + (uint32_t)__builtin_ctzll( hit );
-      *block = low;
+      const uint32_t which = (uint32_t)__builtin_ctzll( hit );
+      found->seq = i0 + which;
+      found->block = low - (uint32_t)__builtin_amdgcn_readlane( (int)first, (int)which );
+      if ( i0 == 0 ) {
+        found->row0 = (uint32_t)__builtin_amdgcn_readlane( (int)my_row0, (int)which );
+        found->tokens = (uint32_t)__builtin_amdgcn_readlane( (int)my_tokens, (int)which );
+        found->start = (uint32_t)__builtin_amdgcn_readlane( (int)my_start, (int)which );
+      } else {
+        found->row0 = s.begin( found->seq );
+        found->tokens = s.count( found->seq );
+        found->start = s.begin_pos( found->seq );
+      }
       return true;
     }
     rank -= n;
