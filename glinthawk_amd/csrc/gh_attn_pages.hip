@@ -503,6 +503,28 @@ __device__ __forceinline__ void read_values( const uint32_t* at, v4s ( *v )[2] )
                 : "memory" );
 }
 
+// a lane's chunk of eight groups of rows, 1 KB apart
+template<uint32_t FIRST, bool WAIT>
+__device__ __forceinline__ void read_rows( uint32_t at, mfma_f32x4 ( &v )[8] )
+{
+  if constexpr ( WAIT ) {
+    asm volatile( "s_waitcnt vmcnt(16)" ::: "memory" );
+  }
+  asm volatile( "ds_read_b128 %0, %8 offset:%9\n\t"
+                "ds_read_b128 %1, %8 offset:%10\n\t"
+                "ds_read_b128 %2, %8 offset:%11\n\t"
+                "ds_read_b128 %3, %8 offset:%12\n\t"
+                "ds_read_b128 %4, %8 offset:%13\n\t"
+                "ds_read_b128 %5, %8 offset:%14\n\t"
+                "ds_read_b128 %6, %8 offset:%15\n\t"
+                "ds_read_b128 %7, %8 offset:%16\n\t"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"( v[0] ), "=&v"( v[1] ), "=&v"( v[2] ), "=&v"( v[3] ), "=&v"( v[4] ), "=&v"( v[5] ), "=&v"( v[6] ), "=&v"( v[7] )
+                : "v"( at ), "n"( FIRST ), "n"( FIRST + 1024 ), "n"( FIRST + 2048 ), "n"( FIRST + 3072 ), "n"( FIRST + 4096 ), "n"( FIRST + 5120 ), "n"( FIRST + 6144 ),
+                  "n"( FIRST + 7168 )
+                : "memory" );
+}
+
 // A stage's values as the first operand of O^T += V^T P^T
 template<typename E, uint32_t NB, uint32_t NU>
 struct Values
@@ -833,6 +855,190 @@ template<typename E, int CH, int W, int HW>
 __global__ __launch_bounds__( 64 * W * HW ) void attn_pages_decode_kernel( const E* __restrict__ q, E* __restrict__ out, Call a )
 {
   decode_run<E, CH, W, HW>( q, out, a );
+}
+
+// =================================================================================================
+// decode in fp32 with one query head a kv head, heads of up to CH chunks of 16 bytes: the same walk, products in the vector ALU
+//
+// One column leaves 15 of the matrix instruction's 16 idle, at 32 cycles each, and where few contexts make a wave's stages a chain those are what it waits for.
+// A lane has chunk lane % CH of rows lane / CH, + 64 / CH, ...: a key's score is 4 products and a sum over CH lanes, its values 4 products of the lane's own dims.
+// 16 contexts of 33 to 1023 keys, 12 heads of 64: 18.8 us in matrix instructions.
+// =================================================================================================
+// sum over the CH (16 or 32) lanes that share a row, in all of them
+template<int CH>
+__device__ __forceinline__ float lanes_sum( float v )
+{
+  v = row16_sum( v );
+  return CH == 32 ? sum_rows( v, v ) : v;
+}
+
+template<int CH, int W>
+__device__ __forceinline__ void decode_run_one( const float* __restrict__ q, float* __restrict__ out, const Call& a )
+{
+  constexpr uint32_t KEYS = 512 / CH, RPI = 64 / CH, LOADS = KEYS / RPI; // 8 loads for a stage's K, and for its V
+  constexpr uint32_t TILE = KEYS * CH * 16;                              // bytes
+  static_assert( LOADS == 8 && TILE == 8192, "" );
+  __shared__ mfma_f32x4 s_tiles[W][4][KEYS * CH]; // of every wave: K of even and of odd stages, V of even and of odd stages
+
+  const uint32_t wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 ), lane = threadIdx.x & 63, c = lane % CH, r = lane / CH;
+  Block b;
+  if ( !block_of<true, 16>( a, blockIdx.x / a.n_kv_heads, blockIdx.x % a.n_kv_heads, blockIdx.y, &b ) ) {
+    return;
+  }
+  const uint32_t length = b.start + 1, k_begin = b.split * a.chunk, k_end = min( length, k_begin + a.chunk );
+  if ( k_begin >= k_end ) {
+    return;
+  }
+  const uint64_t place = (uint64_t)b.row0 * a.n_kv_heads + b.h;
+  const bool ok = 4 * c < a.size; // the lane's chunk is one of the head's
+  const mfma_f32x4 qd = ok ? *reinterpret_cast<const mfma_f32x4*>( q + place * a.size + 4 * c ) : mfma_f32x4 {};
+  const uint32_t at = ok ? r * a.pages.row_bytes + 16 * c : 0x80000000u, k_off = b.h * a.size * 4, v_off = ( a.n_kv_heads + b.h ) * a.size * 4;
+
+  const uint32_t n_stages = ( k_end - k_begin + KEYS - 1 ) / KEYS, n_mine = n_stages > wave ? ( n_stages - wave + W - 1 ) / W : 0;
+  typedef const uint32_t __attribute__( ( address_space( 4 ) ) ) * scalar_ptr;
+  const scalar_ptr table = (scalar_ptr)( reinterpret_cast<uintptr_t>( a.pages.table + (uint64_t)b.seq * a.pages.table_stride ) );
+  constexpr uint32_t NU = KEYS / 16;
+  uint32_t id[NU];
+  auto look_up = [&]( uint32_t stage ) __attribute__( ( always_inline ) ) {
+#pragma unroll
+    for ( uint32_t u = 0; u < NU; u++ ) {
+      id[u] = table[min( k_begin + KEYS * ( stage * W + wave ) + 16 * u, k_end - 1 ) >> a.pages.shift];
+    }
+  };
+  __amdgpu_buffer_rsrc_t rsrc[NU];
+  auto describe = [&]( uint32_t stage ) __attribute__( ( always_inline ) ) {
+#pragma unroll
+    for ( uint32_t u = 0; u < NU; u++ ) {
+      const uint32_t key = k_begin + KEYS * ( stage * W + wave ) + 16 * u;
+      const char* base = a.pages.pool + min( id[u], a.pages.last ) * a.pages.stride + (uint64_t)( key & ( ( 1u << a.pages.shift ) - 1 ) ) * a.pages.row_bytes;
+      const uint32_t rows = key < k_end ? min( k_end - key, 16u ) : 0u;
+      rsrc[u] = __builtin_amdgcn_make_buffer_rsrc( const_cast<char*>( base ), 0, (int)( rows * a.pages.row_bytes ), 0x00020000 );
+    }
+    look_up( stage + 1 );
+  };
+  auto fetch = [&]( mfma_f32x4* tile, uint32_t off ) __attribute__( ( always_inline ) ) {
+#pragma unroll
+    for ( uint32_t t = 0; t < LOADS; t++ ) { // rows RPI t + r
+      __builtin_amdgcn_raw_ptr_buffer_load_lds( rsrc[RPI * t / 16], (lds_ptr)( tile + RPI * t * CH ), 16, at, RPI * t % 16 * a.pages.row_bytes + off, 0, 2 );
+    }
+  };
+  mfma_f32x4 acc = {}; // dims 4 c .. 4 c + 3, of rows r
+  float m = -INFINITY, l = 0.0f; // m: of the wave; l: of rows r
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_ptr)&s_tiles[wave][0][0] + 16 * lane;
+  auto stage = [&]( uint32_t j, auto buffer ) __attribute__( ( always_inline ) ) {
+    constexpr uint32_t B = decltype( buffer )::value;
+    mfma_f32x4 k[8], v[8];
+    read_rows<B * TILE, true>( lds, k ); // all but the 16 loads of stage j + 1 have landed
+    __builtin_amdgcn_sched_barrier( 0 );
+    describe( j + 2 );
+    fetch( s_tiles[wave][B], k_off );
+    const uint32_t key0 = k_begin + KEYS * ( j * W + wave );
+    float s[8], mx = -INFINITY;
+#pragma unroll
+    for ( uint32_t t = 0; t < 8; t++ ) {
+      s[t] = lanes_sum<CH>( __builtin_fmaf( k[t][0], qd[0], k[t][1] * qd[1] ) + __builtin_fmaf( k[t][2], qd[2], k[t][3] * qd[3] ) );
+      s[t] = key0 + RPI * t + r < k_end ? s[t] * a.scale_log2e : -INFINITY;
+      mx = fmaxf( mx, s[t] );
+    }
+    mx = wave_max( mx );
+    if ( mx > m + LAZY ) { // the whole wave
+      const float alpha = fast_exp2( m - mx );
+      m = mx;
+      l *= alpha;
+      acc *= alpha;
+    }
+    const float ms = m == -INFINITY ? 0.0f : m;
+    read_rows<( 2 + B ) * TILE, false>( lds, v );
+    __builtin_amdgcn_sched_barrier( 0 );
+    fetch( s_tiles[wave][2 + B], v_off );
+#pragma unroll
+    for ( uint32_t t = 0; t < 8; t++ ) {
+      const float p = fast_exp2( s[t] - ms );
+      l += p;
+#pragma unroll
+      for ( int e = 0; e < 4; e++ ) {
+        acc[e] = __builtin_fmaf( p, v[t][e], acc[e] );
+      }
+    }
+  };
+  if ( n_mine != 0 ) {
+    look_up( 0 );
+    describe( 0 );
+    fetch( s_tiles[wave][0], k_off );
+    fetch( s_tiles[wave][2], v_off );
+    describe( 1 );
+    fetch( s_tiles[wave][1], k_off );
+    fetch( s_tiles[wave][3], v_off );
+    for ( uint32_t j = 0; j < n_mine; j += 2 ) { // (loads past the end fetch nothing, so that the count of those on their way stays the same)
+      stage( j, std::integral_constant<uint32_t, 0> {} );
+      if ( j + 1 < n_mine ) {
+        stage( j + 1, std::integral_constant<uint32_t, 1> {} );
+      }
+    }
+  }
+  __builtin_amdgcn_s_waitcnt( 0x0F70 ); // vmcnt(0): nothing is on its way to LDS any more
+  // the rows r added up, into all lanes
+  auto rows_sum = [&]( float x ) { return CH == 16 ? column_sum( x ) : sum_halves( x, x ); };
+  l = rows_sum( l );
+#pragma unroll
+  for ( int e = 0; e < 4; e++ ) {
+    acc[e] = rows_sum( acc[e] );
+  }
+  if constexpr ( W > 1 ) { // and the waves, by wave 0
+    mfma_f32x4* parts = &s_tiles[0][0][0];
+    float* ml = reinterpret_cast<float*>( parts + W * CH );
+    __syncthreads();
+    if ( r == 0 ) {
+      parts[wave * CH + c] = acc;
+    }
+    if ( lane == 0 ) {
+      ml[2 * wave] = m;
+      ml[2 * wave + 1] = l;
+    }
+    __syncthreads();
+    if ( wave != 0 ) {
+      return;
+    }
+    float mm = m;
+#pragma unroll
+    for ( int w = 1; w < W; w++ ) {
+      mm = fmaxf( mm, ml[2 * w] );
+    }
+    const float mm_safe = mm == -INFINITY ? 0.0f : mm, w0 = fast_exp2( m - mm_safe );
+    m = mm;
+    l *= w0;
+    acc *= w0;
+#pragma unroll
+    for ( int w = 1; w < W; w++ ) {
+      const float ww = fast_exp2( ml[2 * w] - mm_safe );
+      l = __builtin_fmaf( ml[2 * w + 1], ww, l );
+      const mfma_f32x4 other = parts[w * CH + c];
+#pragma unroll
+      for ( int e = 0; e < 4; e++ ) {
+        acc[e] = __builtin_fmaf( other[e], ww, acc[e] );
+      }
+    }
+  }
+  if ( r != 0 || !ok ) {
+    return;
+  }
+  const uint64_t slot = place * a.splits + b.split;
+  if ( a.splits > 1 ) {
+    *reinterpret_cast<mfma_f32x4*>( a.part_out + slot * a.size + 4 * c ) = acc;
+    if ( lane == 0 ) {
+      a.part_ml[slot * 2] = m;
+      a.part_ml[slot * 2 + 1] = l;
+    }
+  } else {
+    const float inv = 1.0f / l;
+    store4( out + place * a.size + 4 * c, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv );
+  }
+}
+
+template<int CH, int W>
+__global__ __launch_bounds__( 64 * W ) void attn_pages_decode_one_kernel( const float* __restrict__ q, float* __restrict__ out, Call a )
+{
+  decode_run_one<CH, W>( q, out, a );
 }
 
 // =================================================================================================
@@ -1585,6 +1791,17 @@ void launch_decode_tiles( const Plan& p, const Call& a, const void* q, void* out
 {
   const E* tq = static_cast<const E*>( q );
   E* to = static_cast<E*>( out );
+  if constexpr ( sizeof( E ) == 4 ) {
+    if ( a.gqa == 1 ) {
+      const dim3 grid( p.blocks * a.n_kv_heads, p.splits );
+      if ( a.size <= 64 ) {
+        p.waves > 1 ? attn_pages_decode_one_kernel<16, 4><<<grid, 256, 0, st>>>( tq, to, a ) : attn_pages_decode_one_kernel<16, 1><<<grid, 64, 0, st>>>( tq, to, a );
+      } else {
+        p.waves > 1 ? attn_pages_decode_one_kernel<32, 4><<<grid, 256, 0, st>>>( tq, to, a ) : attn_pages_decode_one_kernel<32, 1><<<grid, 64, 0, st>>>( tq, to, a );
+      }
+      return;
+    }
+  }
   auto go = [&]( auto chunks, auto waves, auto heads ) {
     constexpr int CH = decltype( chunks )::value, W = decltype( waves )::value, HW = decltype( heads )::value;
     attn_pages_decode_kernel<E, CH, W, HW><<<dim3( p.blocks * ( a.n_kv_heads / HW ), p.splits ), 64 * W * HW, 0, st>>>( tq, to, a );
