@@ -211,6 +211,8 @@ __global__ __launch_bounds__( THREADS, THREADS >= 512 ? ( THREADS == 512 || PIEC
       rank += other > mine || ( other == mine && w < lane );
     }
     const float reach = lane_value( mine, __builtin_ctzll( __builtin_amdgcn_ballot_w64( rank == WAVES / 2 - 1 ) ) );
+    uint32_t thread = threadIdx.x;
+    asm volatile( "" : "+v"( thread ) ); // (the columns' numbers are made here and not ahead of time)
     if ( !( best < reach ) ) { // few threads come this far
 #pragma unroll
       for ( int p = 0; p < PIECES; p++ ) {
@@ -218,7 +220,7 @@ __global__ __launch_bounds__( THREADS, THREADS >= 512 ? ( THREADS == 512 || PIEC
 #pragma unroll
           for ( int e = 0; e < V; e++ ) {
             const float v = to_f32( piece[p].e[e] );
-            const uint32_t i = ( p * THREADS + threadIdx.x ) * V + e;
+            const uint32_t i = ( p * THREADS + thread ) * V + e;
             if ( !( v < reach ) && i < n ) { // (NaN comes along: where there is nothing else it is wanted)
               const uint32_t at = atomicAdd( &s_count, 1u ); // (their order does not matter: each is ranked among all)
               if ( at < CANDIDATES ) {
