@@ -381,7 +381,7 @@ __global__ __launch_bounds__( 256 ) void attn_pages_f32_kernel( const T* __restr
 // decode, heads of up to CH chunks of 16 bytes: wave <-> (context, kv head, 16 columns, run of keys)
 //
 // Bound by the bytes of the cache.  A wave goes through stages of 32 keys on its own: their K and V rows go from memory straight to its part of LDS, two stages deep,
-// so that a stage (16 KB at 128 elements) is always on its way while one is computed.  Rows behind the keys, and chunks behind a smaller head, lie outside the
+// so that a stage (16 KB at 128 16-bit elements) is always on its way while one is computed.  Rows behind the keys, and chunks behind a smaller head, lie outside the
 // descriptor of their 16 rows (which lie in one page) and arrive as zeros, whatever memory holds there.
 //   S^T = K Q^T     16 x 16 x 32: a lane gets keys 4 g + i (and 16 + 4 g + i) of column c
 //   O^T += V^T P^T  16 x 16 x 32: the weights are the second operand as they lie, if slot 8 g + e is key 4 g + e (e < 4) and 16 + 4 g + e - 4; the first operand's
@@ -439,26 +439,38 @@ __device__ __forceinline__ void store4( E* to, float a, float b, float c, float 
   }
 }
 
+template<uint32_t FIRST, typename Chunk>
+__device__ __forceinline__ void read_chunks( const uint32_t* at, Chunk ( &k )[8] )
+{
+  asm volatile( "ds_read_b128 %0, %8 offset:%16\n\t"
+                "ds_read_b128 %1, %9 offset:%16\n\t"
+                "ds_read_b128 %2, %10 offset:%16\n\t"
+                "ds_read_b128 %3, %11 offset:%16\n\t"
+                "ds_read_b128 %4, %12 offset:%16\n\t"
+                "ds_read_b128 %5, %13 offset:%16\n\t"
+                "ds_read_b128 %6, %14 offset:%16\n\t"
+                "ds_read_b128 %7, %15 offset:%16\n\t"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"( k[0] ), "=&v"( k[1] ), "=&v"( k[2] ), "=&v"( k[3] ), "=&v"( k[4] ), "=&v"( k[5] ), "=&v"( k[6] ), "=&v"( k[7] )
+                : "v"( at[0] ), "v"( at[1] ), "v"( at[2] ), "v"( at[3] ), "v"( at[4] ), "v"( at[5] ), "v"( at[6] ), "v"( at[7] ), "n"( FIRST )
+                : "memory" );
+}
+
 // LDS reads of a stage, written out, each block with its waits: the compiler cannot tell the tiles that a read may take from the ones on their way, and would wait
 // for all of them.
 template<int CH, uint32_t FIRST, uint32_t SECOND, typename Chunk, uint32_t NU>
 __device__ __forceinline__ void read_keys( const uint32_t* at, Chunk ( &k )[NU][CH / 4] )
 {
   if constexpr ( CH == 32 ) {
-    static_assert( NU == 1, "" );
-    asm volatile( "s_waitcnt vmcnt(16)\n\t"
-                  "ds_read_b128 %0, %8 offset:%16\n\t"
-                  "ds_read_b128 %1, %9 offset:%16\n\t"
-                  "ds_read_b128 %2, %10 offset:%16\n\t"
-                  "ds_read_b128 %3, %11 offset:%16\n\t"
-                  "ds_read_b128 %4, %12 offset:%16\n\t"
-                  "ds_read_b128 %5, %13 offset:%16\n\t"
-                  "ds_read_b128 %6, %14 offset:%16\n\t"
-                  "ds_read_b128 %7, %15 offset:%16\n\t"
-                  "s_waitcnt lgkmcnt(0)"
-                  : "=&v"( k[0][0] ), "=&v"( k[0][1] ), "=&v"( k[0][2] ), "=&v"( k[0][3] ), "=&v"( k[0][4] ), "=&v"( k[0][5] ), "=&v"( k[0][6] ), "=&v"( k[0][7] )
-                  : "v"( at[0] ), "v"( at[1] ), "v"( at[2] ), "v"( at[3] ), "v"( at[4] ), "v"( at[5] ), "v"( at[6] ), "v"( at[7] ), "n"( FIRST )
-                  : "memory" );
+    if constexpr ( NU == 1 ) {
+      asm volatile( "s_waitcnt vmcnt(16)" ::: "memory" );
+    } else {
+      asm volatile( "s_waitcnt vmcnt(32)" ::: "memory" );
+    }
+    read_chunks<FIRST>( at, k[0] );
+    if constexpr ( NU == 2 ) {
+      read_chunks<SECOND>( at, k[1] );
+    }
   } else if constexpr ( CH == 16 ) {
     asm volatile( "s_waitcnt vmcnt(16)\n\t"
                   "ds_read_b128 %0, %8 offset:%12\n\t"
@@ -637,7 +649,7 @@ __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restri
   const uint32_t ld_row = lane / CH, ld_slot = lane % CH, chunks = a.size / PER;
   const uint32_t k_off = b.h * a.size * sizeof( E ), v_off = ( a.n_kv_heads + b.h ) * a.size * sizeof( E );
   auto k_swizzle = []( uint32_t row ) { return CH >= 16 ? row & 15 : ( row >> 1 ) & 7; };
-  auto v_swizzle = []( uint32_t row ) { return F32 ? row & 12 : CH == 16 ? 2 * ( row & 7 ) : 2 * ( ( row >> 1 ) & 3 ); };
+  auto v_swizzle = []( uint32_t row ) { return F32 ? row & 12 : CH >= 16 ? 2 * ( row & 7 ) : 2 * ( ( row >> 1 ) & 3 ); };
   uint32_t k_at[IPG], v_at[IPG];
 #pragma unroll
   for ( uint32_t t = 0; t < IPG; t++ ) {
@@ -1119,8 +1131,8 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
   // a lane's place in the rows of a load; chunks behind the head far outside every descriptor
   const uint32_t ld_row = lane / CH, ld_slot = lane % CH, chunks = a.size / 8;
   const uint32_t k_off = h * a.size * 2, v_off = ( a.n_kv_heads + h ) * a.size * 2;
-  auto k_swizzle = []( uint32_t row ) { return CH == 16 ? row & 15 : ( row >> 1 ) & 7; };
-  auto v_swizzle = []( uint32_t row ) { return CH == 16 ? 4 * ( row & 3 ) : 4 * ( ( row >> 1 ) & 1 ); };
+  auto k_swizzle = []( uint32_t row ) { return CH >= 16 ? row & 15 : ( row >> 1 ) & 7; };
+  auto v_swizzle = []( uint32_t row ) { return CH >= 16 ? 4 * ( row & 3 ) : 4 * ( ( row >> 1 ) & 1 ); };
   uint32_t k_at[IPG], v_at[IPG];
 #pragma unroll
   for ( uint32_t t = 0; t < IPG; t++ ) {
@@ -1284,7 +1296,7 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
       }
       if ( n < NP / 2 ) { // vector ALU work beside the matrix units
 #pragma unroll
-        for ( int e0 = 8 / I4 * i4; e0 < 8 / I4 * ( i4 + 1 ); e0 += 2 ) {
+        for ( int e0 = ( 8 * i4 / I4 + 1 ) / 2 * 2; e0 < 8 * ( i4 + 1 ) / I4; e0 += 2 ) { // the pair, pairs or half of the steps a pair
           weights( 2 + kk, e0 );
         }
       }
@@ -1351,7 +1363,7 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
 }
 
 template<typename E, int CH>
-__global__ __launch_bounds__( 256, 2 ) void attn_pages_packed_kernel( const E* __restrict__ q, E* __restrict__ out, Call a )
+__global__ __launch_bounds__( 256, CH == 32 ? 1 : 2 ) void attn_pages_packed_kernel( const E* __restrict__ q, E* __restrict__ out, Call a )
 {
   packed_run<E, CH>( q, out, a );
 }
@@ -1686,7 +1698,7 @@ struct Plan
 };
 
 // The kernels that stream to LDS take heads made of 16-byte chunks, runs of 16 keys in one page, and everything aligned to 16 bytes.
-bool takes_tiles( const gh_shape* s, gh_dtype dt ) { return s->head_size * dtype_size( dt ) % 16 == 0 && s->head_size <= 128; }
+bool takes_tiles( const gh_shape* s, gh_dtype dt ) { return s->head_size * dtype_size( dt ) % 16 == 0 && s->head_size <= ( dt == GH_F32 ? 128 : 256 ); }
 
 constexpr uint64_t MOST_PARTS = 65536; // of (query row, head, split) that leave partial results
 
@@ -1712,10 +1724,11 @@ Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, c
     // 16 x 500, 4 waves 9.8, one wave 15.1 | 64 x 4096, splits of 2048 167, of 512 185, of 64 261 | 256 x 1000, one wave 162, 4 waves 177
     // 32 heads of one query: 8 x 2000, 4 waves 42, one wave 48 | 3 x 30000, splits of 1024 233, of 128 248, 4 waves unsplit 269
     const uint64_t streams = batch * p.n_blocks * s->n_kv_heads;
-    const double slots = 4.0 * cu_count() * ( dt != GH_F32 && s->head_size <= 64 ? 2 : 1 );
+    const bool wide = s->head_size > 128; // twice the bytes and the LDS
+    const double slots = cu_count() * ( wide ? 2.0 : dt != GH_F32 && s->head_size <= 64 ? 8.0 : 4.0 );
     const uint32_t stage = dt == GH_F32 && s->head_size > 64 ? 16 : 32; // keys
     double best = 0;
-    for ( uint32_t waves = 1; waves <= 4; waves += 3 ) {
+    for ( uint32_t waves = 1; waves <= ( wide ? 2 : 4 ); waves += wide ? 1 : 3 ) {
       for ( uint32_t chunk = 64; chunk != 0; chunk = chunk >= max_keys ? 0 : 2 * chunk ) {
         const uint64_t splits = ( max_keys + chunk - 1 ) / chunk;
         if ( splits > 65535 || ( splits > 1 && rows * s->n_heads * splits > MOST_PARTS ) ) {
@@ -1821,8 +1834,14 @@ void launch_decode_tiles( const Plan& p, const Call& a, const void* q, void* out
   constexpr int NARROW = 4 * sizeof( E ); // chunks of 64 elements
   if ( a.size <= 64 ) {
     sizes( std::integral_constant<int, NARROW> {} );
-  } else {
+  } else if ( a.size <= 128 ) {
     sizes( std::integral_constant<int, 2 * NARROW> {} );
+  } else if constexpr ( sizeof( E ) == 2 ) { // 64 KB of LDS a wave
+    if ( p.waves > 1 ) {
+      go( std::integral_constant<int, 32> {}, two, one );
+    } else {
+      go( std::integral_constant<int, 32> {}, one, one );
+    }
   }
 }
 
@@ -1840,8 +1859,10 @@ void launch_packed_tiles( const Plan& p, const Call& a, const void* q, void* out
     }
   } else if ( a.size <= 64 ) {
     attn_pages_packed_kernel<E, 8><<<grid, 256, 0, st>>>( static_cast<const E*>( q ), static_cast<E*>( out ), a );
-  } else {
+  } else if ( a.size <= 128 ) {
     attn_pages_packed_kernel<E, 16><<<grid, 256, 0, st>>>( static_cast<const E*>( q ), static_cast<E*>( out ), a );
+  } else {
+    attn_pages_packed_kernel<E, 32><<<grid, 256, 0, st>>>( static_cast<const E*>( q ), static_cast<E*>( out ), a );
   }
 }
 

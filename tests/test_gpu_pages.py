@@ -64,7 +64,7 @@ def test_decode_pages(page, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
-@pytest.mark.parametrize("heads,kv_heads,size", [(8, 1, 128), (2, 2, 64), (3, 1, 36), (4, 1, 200)])
+@pytest.mark.parametrize("heads,kv_heads,size", [(8, 1, 128), (2, 2, 64), (3, 1, 36), (4, 1, 200), (5, 1, 256), (4, 4, 136)])
 def test_decode_of_long_contexts_in_splits(heads, kv_heads, size, dtype):
     lengths = [3001, 257, 1, 0, 1024, 2047]
     check_decode(Pool(lengths, kv_heads, size, dtype, 32), heads, lengths)
@@ -159,7 +159,7 @@ def test_packed_pages(page, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
-@pytest.mark.parametrize("heads,kv_heads,size", [(8, 1, 128), (2, 2, 64), (3, 1, 36)])
+@pytest.mark.parametrize("heads,kv_heads,size", [(8, 1, 128), (2, 2, 64), (3, 1, 36), (3, 1, 256), (2, 2, 136)])
 def test_packed_over_many_stages_and_splits(heads, kv_heads, size, dtype):
     tokens, start = [300, 2, 129], [0, 1500, 700]
     check_packed(Pool([n + s for n, s in zip(tokens, start)], kv_heads, size, dtype, 32), heads, tokens, start)
@@ -172,7 +172,7 @@ def test_packed_many_sequences(dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
-@pytest.mark.parametrize("heads,kv_heads,size", [(8, 1, 128), (2, 2, 128), (2, 1, 64), (3, 1, 36)])
+@pytest.mark.parametrize("heads,kv_heads,size", [(8, 1, 128), (2, 2, 128), (2, 1, 64), (3, 1, 36), (2, 1, 200)])
 @pytest.mark.parametrize("start", [0, 900])
 def test_what_stands_behind_a_token_does_not_reach_it(heads, kv_heads, size, dtype, start):
     """Infinities and NaN in a later token's row: the tokens before it are as if they were not there, those from it on are what the formula gives."""
