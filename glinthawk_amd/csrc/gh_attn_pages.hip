@@ -1191,7 +1191,8 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
   next = describe( 1, look_up( 1 ) ); // of stage i + 1
   fetch( next, s_k1, k_at );
   uint32_t id = look_up( 2 ); // of stage i + 2
-  __builtin_amdgcn_s_waitcnt( 0x0F70 ); // vmcnt(0)
+  // the first stage's keys have landed; its values and the second's keys (2 IPG loads) are waited for at the top of the loop
+  __builtin_amdgcn_s_waitcnt( CH == 32 ? 0x4F70 : CH == 16 ? 0x0F78 : 0x0F74 );
   __syncthreads();
   mfma_f32x16 st_a[2], st_b[2]; // scores of even and of odd stages
   if ( my_stages > 0 ) {
@@ -1283,6 +1284,7 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
         weights( kk, e0 );
       }
     }
+    __builtin_amdgcn_s_setprio( 1 ); // before the other wave of the SIMD while this one has matrix work: their softmaxes fall beside it (4096 tokens: 300 us, so 295)
     __builtin_amdgcn_sched_barrier( 0 );
 #pragma unroll
     for ( int n = 0; n < NP; n++ ) {
@@ -1302,6 +1304,7 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
       }
       __builtin_amdgcn_sched_barrier( 0 );
     }
+    __builtin_amdgcn_s_setprio( 0 );
     l += sum[0] + sum[1];
   };
   for ( uint32_t i = 0; i < n_stages; i += 2 ) {

@@ -171,6 +171,11 @@ int gh_copy_pages_host( void* pool, uint64_t page_stride, uint64_t page_bytes, u
   }
   constexpr uint64_t PART = STAGE_SLOT_BYTES / 8; // pairs of a staging slot; the pages of different pairs are apart, so parts may follow each other in any order
   hipStream_t st = as_stream( stream );
+  if ( st != nullptr ) { // a graph would copy the pairs from the staging slot again when that holds something else
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    GH_HIP( hipStreamIsCapturing( st, &capture ) );
+    GH_REQUIRE( capture == hipStreamCaptureStatusNone, "gh_copy_pages_host: the stream is being captured into a graph, which takes pairs in device memory" );
+  }
   for ( uint64_t j = 0; j < n_pairs; j += PART ) {
     const uint64_t n = std::min( PART, n_pairs - j );
     StageScope scope( st );

@@ -409,7 +409,8 @@ int gh_attn_packed( const void* q, const gh_pages* pages, const uint32_t* first_
                     uint32_t max_keys, const gh_shape* shape, gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream );
 /* Pages copied within a pool, in each of `layers` layers (layer k's pages begin layer_stride bytes behind those of k - 1): page pairs[2 j + 1] becomes a copy of
  * page pairs[2 j], page_bytes bytes of it.  A pair with a number that is not below n_pages is left out.  No page may be written twice, or be both written and read, in
- * one call: the host form checks it, and the numbers, and refuses; the plain form's pairs are in device memory and are the caller's to keep apart. */
+ * one call: the host form checks it, and the numbers, and refuses, as it does a
+ * stream under capture; the plain form's pairs are in device memory and are the caller's to keep apart. */
 int gh_copy_pages( void* pool, uint64_t page_stride, uint64_t page_bytes, uint32_t n_pages, uint64_t layers, uint64_t layer_stride, const uint32_t* pairs_dev,
                    uint64_t n_pairs, gh_stream stream );
 int gh_copy_pages_host( void* pool, uint64_t page_stride, uint64_t page_bytes, uint32_t n_pages, uint64_t layers, uint64_t layer_stride, const uint32_t* pairs_host,

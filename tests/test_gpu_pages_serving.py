@@ -180,6 +180,24 @@ def test_graphs_that_are_replayed(dtype):
                 assert bool((kept[0][c] == 3.0).all())
 
 
+def test_pairs_in_host_memory_are_not_captured():
+    from glinthawk_amd._lib import GlintError
+
+    pool = torch.arange(6, dtype=torch.float32).cuda()[:, None, None].expand(6, 4, 8).contiguous()
+    pairs, graph = torch.tensor([[0, 3]], dtype=torch.int32).cuda(), torch.cuda.CUDAGraph()
+    ops.copy_pages(pool, [(5, 4)])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        with pytest.raises(GlintError, match="captured"):
+            ops.copy_pages(pool, [(1, 2)])
+        ops.copy_pages(pool, pairs)
+    for source in (1, 2, 0):
+        pairs[0, 0] = source
+        graph.replay()
+        torch.cuda.synchronize()
+        assert pool[:, 0, 0].tolist() == [0, 1, 2, source, 5, 5]
+
+
 def test_two_at_a_time():
     """Two graphs with workspaces of their own, and eager calls on a third stream, at once."""
     made = [parts(i) for i in (1, 2, 3)]
