@@ -594,20 +594,28 @@ int64_t glint_pages_compact( void* b, uint32_t* pairs, uint64_t cap )
 // tokens of a context, -1: not known
 int64_t glint_pages_length( void* b, uint64_t id )
 {
-  const auto context = static_cast<PageBook*>( b )->context( id );
-  return context ? static_cast<int64_t>( context->length ) : -1;
+  try {
+    const auto context = static_cast<PageBook*>( b )->context( id );
+    return context ? static_cast<int64_t>( context->length ) : -1;
+  } catch ( const std::bad_alloc& ) {
+    return -1;
+  }
 }
 // the number of a context's pages, up to cap of them in out; -1: not known
 int64_t glint_pages_line( void* b, uint64_t id, uint32_t* out, uint64_t cap )
 {
-  const auto context = static_cast<PageBook*>( b )->context( id );
-  if ( !context ) {
+  try {
+    const auto context = static_cast<PageBook*>( b )->context( id );
+    if ( !context ) {
+      return -1;
+    }
+    for ( size_t i = 0; i < context->pages.size() && i < cap; i++ ) {
+      out[i] = context->pages[i];
+    }
+    return static_cast<int64_t>( context->pages.size() );
+  } catch ( const std::bad_alloc& ) {
     return -1;
   }
-  for ( size_t i = 0; i < context->pages.size() && i < cap; i++ ) {
-    out[i] = context->pages[i];
-  }
-  return static_cast<int64_t>( context->pages.size() );
 }
 
 // paged context over a counting region: hosts `n_hosted` layers of the 70B-4K shape

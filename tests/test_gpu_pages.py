@@ -77,6 +77,22 @@ def test_decode_of_many_contexts(dtype):
     check_decode(Pool(lengths, 1, 64, dtype), 4, lengths)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("batch", [2, 63, 64, 65])
+def test_decode_in_order_of_length(batch, dtype):
+    """More work-groups than run at a time, lengths that are equal, zero, ascending and beyond the bound: each context once, whatever the order they are taken in."""
+    lengths = [(0, 5, 5, 17 + i, 40, 0, 90 - i)[i % 7] for i in range(batch - 2)] + [1024, 1100]
+    pool = Pool(lengths, 64 if batch > 2 else 1040, 8, dtype)
+    q, xb = decode(pool, pool.kv_heads, lengths, max_length=1024)
+    for i, n in enumerate(lengths):
+        n = min(n, 1024)
+        if n == 0:
+            assert bool((xb[i] == 7.0).all())
+            continue
+        want, off = attention(q[i:i + 1].reshape(1, pool.kv_heads, 8), pool.k(i)[:n], pool.v(i)[:n], n - 1, dtype, dtype != F32)
+        hold(xb[i].reshape(1, pool.kv_heads, 8), want, off, f"context {i} of {n} keys")
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("spare,shift", [(1, 0), (0, 1), (8, 8), (24, 16), (3, 5)])
 def test_pages_that_lie_apart_or_unaligned(spare, shift, dtype):
