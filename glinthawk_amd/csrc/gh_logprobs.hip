@@ -53,18 +53,21 @@ __device__ __forceinline__ uint64_t wave_max_u64( uint64_t v )
   return v;
 }
 
-// the k-th largest value of a wave's lanes (equal ones count each), without NaN; k at most 64
-__device__ __forceinline__ float largest_of( float v, uint32_t k )
+// A value that at least k of a wave's lanes reach, and few more than k: of distances from the largest, the k-th by its upper 16 bits, then the farthest lane within it.
+// v without NaN, k at most 64, largest: of the wave.
+__device__ __forceinline__ float reached_by( float v, float largest, uint32_t k )
 {
-  for ( ;; ) {
-    const float t = wave_max( v );
-    const uint32_t n = (uint32_t)__popcll( __builtin_amdgcn_ballot_w64( v == t ) );
-    if ( n >= k || t == -INFINITY ) {
-      return t;
-    }
-    k -= n;
-    v = v == t ? -INFINITY : v;
+  if ( k == 1 ) {
+    return largest;
   }
+  const uint32_t d = v == largest ? 0u : __builtin_bit_cast( uint32_t, largest - v );
+  uint32_t within = 0x7fffffffu;
+#pragma unroll
+  for ( int bit = 30; bit >= 16; bit-- ) {
+    const uint32_t less = within - ( 1u << bit );
+    within = (uint32_t)__popcll( __builtin_amdgcn_ballot_w64( d <= less ) ) >= k ? less : within;
+  }
+  return -wave_max( d <= within ? -v : -INFINITY );
 }
 
 // 16 bytes of a row
@@ -179,19 +182,28 @@ __global__ __launch_bounds__( THREADS, THREADS >= 512 ? ( THREADS == 512 || PIEC
     best = fmaxf( best, piece_best[p] );
   }
   const float wave_best = wave_max( best );
-  const float wave_reach = n_top == 0 ? 0.0f : largest_of( best, ( n_top + WAVES / 2 - 1 ) / ( WAVES / 2 ) );
+  const float wave_reach = n_top == 0 ? 0.0f : reached_by( best, wave_best, ( n_top + WAVES / 2 - 1 ) / ( WAVES / 2 ) );
   if ( lane == 0 ) {
     s_best[wave] = wave_best;
     s_reach[wave] = wave_reach;
   }
   __syncthreads();
   const float max_m = wave_max( lane < WAVES ? s_best[lane] : -INFINITY ), m = max_m == -INFINITY ? 0.0f : max_m, c = m * LOG2E;
-  float s4[4] = { 0, 0, 0, 0 }, t4[4] = { 0, 0, 0, 0 }; // in powers of 2, relative to 2^c: see `sums_of`
+  // f16: in powers of 2, relative to 2^c (see `sums_of`); larger types' values may lie so far from 0 that c's rounding is a large number
+  constexpr bool SMALL = std::is_same_v<T, __half>;
+  float s4[4] = { 0, 0, 0, 0 }, t4[4] = { 0, 0, 0, 0 };
 #pragma unroll
   for ( int p = 0; p < PIECES; p++ ) {
 #pragma unroll
     for ( int e = 0; e < V; e++ ) {
-      const float d = __builtin_fmaf( to_f32( piece[p].e[e] ), LOG2E, -c ), w = __builtin_amdgcn_exp2f( d ); // one rounding, f16 taken as it is
+      float d, w;
+      if constexpr ( SMALL ) {
+        d = __builtin_fmaf( to_f32( piece[p].e[e] ), LOG2E, -c ); // one rounding, f16 taken as it is
+        w = __builtin_amdgcn_exp2f( d );
+      } else {
+        d = to_f32( piece[p].e[e] ) - m; // exact where it matters
+        w = __builtin_amdgcn_exp2f( d * LOG2E );
+      }
       s4[e & 3] += w;
       t4[e & 3] = __builtin_fmaf( w, fmaxf( d, -1e30f ), t4[e & 3] ); // (a weight of 0 times -inf counts nothing)
     }
@@ -239,7 +251,7 @@ __global__ __launch_bounds__( THREADS, THREADS >= 512 ? ( THREADS == 512 || PIEC
     total.x += s_sums[w].x;
     total.y += s_sums[w].y;
   }
-  const Sums z = sums_of( max_m, m, c, total.x, total.y );
+  const Sums z = SMALL ? sums_of( max_m, m, c, total.x, total.y ) : Sums { max_m, total.x, total.y };
   const uint64_t part = row * gridDim.x + blockIdx.x;
   if ( threadIdx.x == 0 ) {
     if ( gridDim.x == 1 ) {

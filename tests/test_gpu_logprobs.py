@@ -66,6 +66,45 @@ def test_equal_values_masked_values_and_nan(vocab, dtype):
     assert torch.equal(ids[7].long(), logprobs(logits[7:], tokens[7:], 64)[2][0])
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("vocab", [33, 1000, 32000, 40000])
+def test_rows_of_the_largest_and_lowest_values(vocab, dtype):
+    """Whole rows at the ends of the type, where a value times log2(e) leaves fp32, and what is about 1e30 away from 0."""
+    logits = torch.zeros((7, vocab))
+    ends = torch.finfo(dtype)
+    logits[0] = ends.min
+    logits[1] = ends.max
+    logits[2, ::2] = ends.min
+    logits[2, 1::2] = -INF
+    logits[3] = ends.min
+    logits[3, 5] = ends.max
+    big = min(1e30, float(ends.max) / 4)
+    logits[4] = -big
+    logits[4, 7] = -0.7 * big
+    logits[5] = 0.5 * big
+    logits[5, ::3] = 0.6 * big
+    logits[6] = -0.69 * big
+    logits = logits.to(dtype).cuda()
+    given, entropy, ids, values = ops.token_logprobs(logits, torch.full((7,), 7, dtype=torch.int32).cuda(), 20)
+    want = logprobs(logits, torch.full((7,), 7, dtype=torch.int32).cuda(), 20)
+    assert torch.equal(ids.long(), want[2])
+    # equal values have one weight each and the others none, so a row's sums are a whole number n; what is left is the logarithm and the difference to the maximum,
+    # each off by its own step (both below 12 where they are finite in fp32, or the difference is all there is)
+    for got, exact in ((given, want[0]), (entropy, want[1]), (values, want[3])):
+        exact = exact.float().double()
+        assert bool((((got.double() - exact).abs() <= 4 * STEP32 * (12 + exact.abs())) | (got.double() == exact)).all())
+
+
+@pytest.mark.parametrize("vocab", [900, 32000, 40000])
+def test_values_far_from_zero(vocab):
+    g = torch.Generator().manual_seed(9)
+    base = torch.tensor([sign * 10.0 ** e for e in (3, 5, 6, 6.05, 7, 9, 12, 20, 30, 37) for sign in (1, -1)])
+    logits = (base[:, None].double() + 3 * torch.randn((20, vocab), generator=g).double()).float().cuda()
+    tokens = torch.randint(vocab, (20,), generator=g, dtype=torch.int32).cuda()
+    for n_top in (1, 20, 64):
+        check(logits, tokens, n_top)
+
+
 def test_nan_and_infinities_only():
     logits = torch.tensor([[NAN] * 70, [-INF] * 70, [INF] * 2 + [0.0] * 68]).cuda()
     given, entropy, ids, values = ops.token_logprobs(logits, torch.zeros(3, dtype=torch.int32).cuda(), 64)
