@@ -5,9 +5,11 @@
 // All three are kept as a pass goes: where the maximum grows by d, S becomes e^-d S and T becomes e^-d (T - d S).
 //
 // A part of a row is held in the registers of a work-group, so that the logits are read once, all pieces asked for at the start: bound by the bytes for many rows (and
-// nearly by the vector ALU: some 12 slots a value), by latency for few.
-// The largest values: of the threads' own largest, each wave knows the q-th; half the waves have q threads that reach the middle one of those, so with q = 2 n / waves
-// at least n values do, and of many thousand only some more.  They go to LDS as whole numbers, a value's bits in the order of the values, then its index the other way
+// nearly by the vector ALU: some 12 slots a value), by latency for few.  2047 rows of 32000 f16 values, 20 alternatives: 41 us (3.2 TB/s), without alternatives 27 (4.9);
+// 7 rows in fp32, 5 alternatives: 7.7 us.  Sums made piece by piece as the loads land, each thread relative to its own maximum, were no faster (43 us): the
+// work-groups of a CU are in different phases already.
+// The largest values: of the threads' own largest, each wave finds one that q of its threads reach and few more; half the waves have q threads that reach the middle one of
+// those, so with q = 2 n / waves at least n values do, and of many thousand only some more.  They go to LDS as whole numbers, a value's bits in the order of the values, then its index the other way
 // round, so that no two are equal and the lower index of equal values is the larger number, and are ranked by counting; where they are more than fit, the numbers come
 // out one after the other, each the largest below the one before.
 // Rows of one part are finished by their work-group.  Longer ones are cut into parts whose S, T, m and sorted largest numbers a second kernel joins.
@@ -54,6 +56,7 @@ __device__ __forceinline__ uint64_t wave_max_u64( uint64_t v )
 }
 
 // A value that at least k of a wave's lanes reach, and few more than k: of distances from the largest, the k-th by its upper 16 bits, then the farthest lane within it.
+// (64 alternatives of 2047 rows: 50 us; with one maximum after the other 60.)
 // v without NaN, k at most 64, largest: of the wave.
 __device__ __forceinline__ float reached_by( float v, float largest, uint32_t k )
 {
@@ -402,7 +405,7 @@ void launch_logprobs( const LogprobPlan& p, const Outputs& o, const void* logits
   } else if ( pieces <= 2048 ) {
     go( many, std::integral_constant<int, 2> {} );
   } else if ( pieces <= 4096 && std::is_same_v<T, __half> && rows >= 512 ) {
-    // more work-groups a CU, whose short phases fill each other's gaps (2047 rows of 32000, 20 alternatives: 40 us, with 1024 threads 46; 256 rows: 11.0 and 10.2; bf16 does not
+    // more work-groups a CU, whose short phases fill each other's gaps (2047 rows of 32000, 20 alternatives: 40 us, with 1024 threads 46, with 256 43; 256 rows: 11.0 and 10.2; bf16 does not
     // fit the registers so: 47 and 47)
     go( std::integral_constant<int, 512> {}, std::integral_constant<int, 8> {} );
   } else if ( pieces <= 4096 ) {

@@ -41,6 +41,7 @@ __global__ __launch_bounds__( 256 ) void page_rows_kernel( Pages p, Packed s, vo
 }
 
 // grid: (pieces of a page, pairs, layers); P: 16 bytes, or 2 where addresses or sizes are not multiples of 16 (1 where they are odd)
+// Bound by the bytes: 1999 pages of 64 KB in 4 layers 187 us, 5.6 TB/s in and out; by its launch where there are few: 5 such pages in 10 layers 3 us.
 template<typename P>
 __global__ __launch_bounds__( 256 ) void copy_pages_kernel( char* pool, uint64_t stride, uint64_t bytes, uint32_t n_pages, uint64_t layer_stride,
                                                           const uint32_t* __restrict__ pairs, uint32_t n_pairs )

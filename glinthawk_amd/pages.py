@@ -42,6 +42,12 @@ class PageBook:
             raise KeyError(name)
         return self._ids[name]
 
+    @staticmethod
+    def _held(answer: int) -> int:
+        if answer < 0:          # of a context that is known
+            raise MemoryError("no memory for the page book's answer")
+        return answer
+
     def _new(self) -> int:
         self._next += 1
         return self._next
@@ -75,23 +81,23 @@ class PageBook:
     def compact(self) -> Pairs:
         """Pages in use move to the front of the pool; the copies to make.  Tables made before are out of date."""
         pairs = (C.c_uint32 * (2 * self.n_pages))()
-        n = host_lib().glint_pages_compact(self._b, pairs, self.n_pages)
+        n = self._held(host_lib().glint_pages_compact(self._b, pairs, self.n_pages))
         return [(pairs[2 * i], pairs[2 * i + 1]) for i in range(n)]
 
     def length(self, name: Hashable) -> int:
-        return int(host_lib().glint_pages_length(self._b, self._known(name)))
+        return int(self._held(host_lib().glint_pages_length(self._b, self._known(name))))
 
     def line(self, name: Hashable) -> List[int]:
         n = -(-self.length(name) // self.page_tokens)
         out = (C.c_uint32 * max(n, 1))()
-        host_lib().glint_pages_line(self._b, self._known(name), out, n)
+        self._held(host_lib().glint_pages_line(self._b, self._known(name), out, n))
         return list(out[:n])
 
     def table(self, names: Sequence[Hashable], entries: int) -> np.ndarray:
         """(names, entries) page numbers, 0 behind a context's last."""
         out = np.zeros((len(names), entries), dtype=np.int32)
         for row, name in zip(out, names):
-            n = host_lib().glint_pages_line(self._b, self._known(name), row.ctypes.data_as(C.POINTER(C.c_uint32)), entries)
+            n = self._held(host_lib().glint_pages_line(self._b, self._known(name), row.ctypes.data_as(C.POINTER(C.c_uint32)), entries))
             if n > entries:
                 raise ValueError(f"context {name!r} has {n} pages, the table {entries} entries")
         return out

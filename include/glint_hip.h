@@ -390,7 +390,7 @@ typedef struct gh_pages
 /* Cache rows and positions of the new tokens of packed sequences: tokens [first_dev[i], first_dev[i + 1]) belong to sequence i and stand at positions
  * start_pos_dev[i] and up (start_pos_dev NULL: all 0).  token_rows_out and pos_out (n_tokens each, either may be NULL) are the tables that gh_kv_append,
  * gh_rope and the fused projections take.  A token that no sequence has, or whose position the table does not reach, or whose page number is not below
- * n_pages gets a NULL row, which those ops skip. */
+ * n_pages gets a NULL row, which those ops skip.  (gh_rope's tables are to have a row for every position there is.) */
 int gh_page_rows( const gh_pages* pages, const uint32_t* first_dev, const uint32_t* start_pos_dev, uint64_t batch, uint64_t n_tokens, uint32_t kv_dim,
                   void** token_rows_out, uint32_t* pos_out, gh_dtype dt, gh_stream stream );
 /* gh_attn_decode over pages: query row i attends the keys [0, lengths_dev[i]) of context i, the current token's among them.  Length 0: an empty context,
@@ -409,8 +409,8 @@ int gh_attn_packed( const void* q, const gh_pages* pages, const uint32_t* first_
                     uint32_t max_keys, const gh_shape* shape, gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream );
 /* Pages copied within a pool, in each of `layers` layers (layer k's pages begin layer_stride bytes behind those of k - 1): page pairs[2 j + 1] becomes a copy of
  * page pairs[2 j], page_bytes bytes of it.  A pair with a number that is not below n_pages is left out.  No page may be written twice, or be both written and read, in
- * one call: the host form checks it, and the numbers, and refuses, as it does a
- * stream under capture; the plain form's pairs are in device memory and are the caller's to keep apart. */
+ * one call: the host form checks it, and the numbers, and refuses, as it does a stream under capture; the plain form's pairs are in device memory and are the
+ * caller's to keep apart. */
 int gh_copy_pages( void* pool, uint64_t page_stride, uint64_t page_bytes, uint32_t n_pages, uint64_t layers, uint64_t layer_stride, const uint32_t* pairs_dev,
                    uint64_t n_pairs, gh_stream stream );
 int gh_copy_pages_host( void* pool, uint64_t page_stride, uint64_t page_bytes, uint32_t n_pages, uint64_t layers, uint64_t layer_stride, const uint32_t* pairs_host,
