@@ -2,16 +2,16 @@
 // shares its parent's pages; the first to write into a shared last page gets a copy of it.  Integers only: the copies that a call asks for come back as pairs
 // (source, destination), for gh_copy_pages to carry out before anything is written to or read from the pages that moved.
 //   - the free page with the lowest number is taken first
-//   - a call that cannot be served changes nothing
+//   - a call that cannot be served, for want of pages or of memory, changes nothing
 //   - the pairs of one call never name a page twice among the destinations, nor one as source and destination.  That holds for pairs of several calls
 //     only while nothing is released or compacted between them, so they are carried out first
 // No counterpart in the reference, whose contexts are one run of rows each.
 #pragma once
 
+#include <algorithm>
 #include <cstdint>
 #include <mutex>
 #include <optional>
-#include <set>
 #include <unordered_map>
 #include <utility>
 #include <vector>
@@ -31,17 +31,15 @@ public:
   PageBook( const uint32_t n_pages, const uint32_t page_tokens )
     : page_tokens_( page_tokens )
     , users_( n_pages, 0 )
+    , n_free_( n_pages )
   {
-    for ( uint32_t p = 0; p < n_pages; p++ ) {
-      free_.insert( free_.end(), p );
-    }
   }
 
   // Room for `tokens` more tokens of a context, which begins here if it is not known; the copies to make, or nothing if the pages do not suffice.
   std::optional<std::vector<Pair>> extend( const uint64_t id, const uint64_t tokens )
   {
     std::lock_guard lock { mutex_ };
-    const auto known = contexts_.find( id );
+    auto known = contexts_.find( id );
     const uint64_t length = known == contexts_.end() ? 0 : known->second.length;
     const uint64_t have = known == contexts_.end() ? 0 : known->second.pages.size();
     if ( tokens > MOST_TOKENS || length + tokens > MOST_TOKENS ) {
@@ -49,13 +47,19 @@ public:
     }
     const bool copy = tokens > 0 && length % page_tokens_ != 0 && users_[known->second.pages.back()] > 1;
     const uint64_t want = ( length + tokens + page_tokens_ - 1 ) / page_tokens_ - have;
-    if ( want + ( copy ? 1 : 0 ) > free_.size() ) {
+    if ( want + ( copy ? 1 : 0 ) > n_free_ ) {
       return std::nullopt;
     }
     std::vector<Pair> pairs;
     pairs.reserve( 1 ); // what could fail comes before the first change
-    auto& context = contexts_[id];
-    context.pages.reserve( have + want );
+    if ( known == contexts_.end() ) {
+      Context fresh;
+      fresh.pages.reserve( want );
+      known = contexts_.emplace( id, std::move( fresh ) ).first;
+    } else {
+      known->second.pages.reserve( have + want );
+    }
+    auto& context = known->second;
     if ( copy ) {
       const uint32_t old = context.pages.back();
       context.pages.back() = take();
@@ -77,11 +81,10 @@ public:
     if ( from == contexts_.end() || contexts_.count( child ) != 0 ) {
       return false;
     }
-    const Context copy = from->second;
-    for ( const uint32_t p : copy.pages ) {
+    const auto& begun = contexts_.emplace( child, Context { from->second } ).first->second; // (what could fail)
+    for ( const uint32_t p : begun.pages ) {
       users_[p]++;
     }
-    contexts_.emplace( child, copy );
     return true;
   }
 
@@ -94,7 +97,7 @@ public:
     }
     for ( const uint32_t p : it->second.pages ) {
       if ( --users_[p] == 0 ) {
-        free_.insert( p );
+        give( p );
       }
     }
     contexts_.erase( it );
@@ -105,26 +108,23 @@ public:
   std::vector<Pair> compact()
   {
     std::lock_guard lock { mutex_ };
-    const uint32_t used = static_cast<uint32_t>( users_.size() - free_.size() );
+    const uint32_t used = static_cast<uint32_t>( users_.size() - n_free_ );
+    std::vector<uint32_t> to( n_free_ ); // of pages from `used` on
     std::vector<Pair> pairs;
-    std::unordered_map<uint32_t, uint32_t> to;
-    for ( uint32_t p = used; p < users_.size(); p++ ) {
+    pairs.reserve( static_cast<size_t>( std::count_if( users_.begin() + used, users_.end(), []( const uint32_t n ) { return n != 0; } ) ) );
+    for ( uint32_t p = used; p < users_.size(); p++ ) { // (nothing fails from here on)
       if ( users_[p] != 0 ) {
         const uint32_t place = take(); // below `used`: as many places are free there as pages are in use beyond
         users_[place] = users_[p];
         users_[p] = 0;
+        give( p );
         pairs.emplace_back( p, place );
-        to.emplace( p, place );
+        to[p - used] = place;
       }
-    }
-    for ( const auto& pair : pairs ) {
-      free_.insert( pair.first );
     }
     for ( auto& [id, context] : contexts_ ) {
       for ( uint32_t& p : context.pages ) {
-        if ( const auto moved = to.find( p ); moved != to.end() ) {
-          p = moved->second;
-        }
+        p = p < used ? p : to[p - used];
       }
     }
     return pairs;
@@ -140,7 +140,7 @@ public:
   [[nodiscard]] uint64_t free() const
   {
     std::lock_guard lock { mutex_ };
-    return free_.size();
+    return n_free_;
   }
 
 private:
@@ -148,16 +148,24 @@ private:
 
   uint32_t take()
   {
-    const uint32_t p = *free_.begin();
-    free_.erase( free_.begin() );
-    users_[p] = 1;
-    return p;
+    while ( users_[lowest_] != 0 ) {
+      lowest_++;
+    }
+    users_[lowest_] = 1;
+    n_free_--;
+    return lowest_++;
+  }
+  void give( const uint32_t p )
+  {
+    n_free_++;
+    lowest_ = std::min( lowest_, p );
   }
 
   mutable std::mutex mutex_ {};
   const uint64_t page_tokens_;
-  std::vector<uint32_t> users_; // contexts a page has
-  std::set<uint32_t> free_ {};
+  std::vector<uint32_t> users_; // contexts a page has; 0: it is free
+  uint32_t n_free_;
+  uint32_t lowest_ { 0 }; // no page below is free
   std::unordered_map<uint64_t, Context> contexts_ {};
 };
 

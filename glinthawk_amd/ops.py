@@ -530,7 +530,9 @@ def copy_pages(pool: torch.Tensor, pairs) -> None:
             _refuse(pool, pairs=(pairs, torch.int32, (pairs.shape[0] if pairs.dim() else 0, 2)))
         check(lib().gh_copy_pages(*common, pairs.data_ptr(), pairs.shape[0], _stream_on(pool.device)), "gh_copy_pages")
     else:
-        flat = [int(v) for pair in pairs for v in pair]
+        flat = [int(v) for source, destination in pairs for v in (source, destination)]
+        if any(not 0 <= v < n_pages for v in flat):
+            raise ValueError(f"pairs that name no page of {n_pages}")
         check(lib().gh_copy_pages_host(*common, host_u32_array(flat), len(flat) // 2, _stream_on(pool.device)), "gh_copy_pages_host")
 
 

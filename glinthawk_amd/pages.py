@@ -56,6 +56,8 @@ class PageBook:
         """Room for `tokens` more tokens; the copies to make, or None, and nothing changed, where the pages do not suffice."""
         if tokens < 0:
             raise ValueError(f"{tokens} tokens")
+        if tokens >= 2 ** 31:
+            return None
         known = self._ids.get(name)
         number = self._new() if known is None else known
         pair = (C.c_uint32 * 2)()

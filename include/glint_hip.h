@@ -377,7 +377,7 @@ int gh_attn_prefill( const void* q, const void* const* layer_rows_dev, const uin
  * [K | V] one behind the other, and every context (or sequence) has a line of page numbers in `table`: its token t lies in row
  * t % page_tokens of page table[context * table_stride + t / page_tokens].  Contexts may have pages in common.  A page number that is not
  * below n_pages reads as the last page: nothing outside the pool is touched, and what such a context gives is not specified.
- * Storage types f16, bf16 and f32; K, V and queries alike.  Head sizes up to 256, any gqa. */
+ * Storage types f16, bf16 and f32; K, V and queries alike.  Head sizes up to 256, any gqa.  Outputs are memory of their own: not q, not the pool. */
 typedef struct gh_pages
 {
   void* pool;               /* this layer's pages; page p begins p * page_stride bytes from here; aligned to its elements */
@@ -418,7 +418,8 @@ int gh_copy_pages_host( void* pool, uint64_t page_stride, uint64_t page_bytes, u
 /* What a caller asks of rows of logits besides gh_argmax: with p = softmax(row), fp32 results
  *   logprob(i) = ln p[tokens_dev[i]] (left as it is where the token is not below vocab);  entropy(i) = - sum p ln p, a value of -inf counting as none;
  *   top_ids, top_logprobs (rows, n_top) = the n_top largest values of the row, largest first, the lower index first among equals, NaN behind everything.
- * logprob with tokens_dev, entropy, and the two of the alternatives may be NULL where they are not wanted (n_top 0).  Rows lie row_stride elements apart; n_top up to 64. */
+ * logprob with tokens_dev, entropy, and the two of the alternatives may be NULL where they are not wanted (n_top 0).  Up to 65535 rows of up to 2097152
+ * values, row_stride elements apart; n_top up to 64.  The workspace as above. */
 uint64_t gh_token_logprobs_workspace( uint64_t rows, uint64_t vocab, uint32_t n_top );
 int gh_token_logprobs( float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs, const void* logits, uint64_t row_stride, const uint32_t* tokens_dev,
                        uint64_t vocab, uint64_t rows, uint32_t n_top, gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream );

@@ -1,8 +1,11 @@
 """Pages of a pool and the contexts that have them: against a plain model of lists and counts, on random runs of calls."""
+import os
 import random
+import subprocess
 
 import pytest
 
+import glinthawk_amd
 from glinthawk_amd.pages import PageBook
 
 
@@ -105,3 +108,79 @@ def test_the_first_to_write_a_shared_page_gets_the_copy():
     book.fork("b", "c")
     assert book.extend("c", 12) == [(1, 2)]          # 21 tokens and 12: to the 33rd
     assert book.line("c") == [0, 2, 3] and book.length("c") == 33
+
+
+FAILING = r"""
+#include "glint/pages.hh"
+#include <cstdio>
+#include <cstdlib>
+#include <new>
+
+static long left = -1; // allocations until one fails; -1: none does
+void* operator new( std::size_t n )
+{
+  if ( left == 0 ) {
+    throw std::bad_alloc {};
+  }
+  left -= left > 0;
+  void* p = std::malloc( n );
+  if ( p == nullptr ) {
+    throw std::bad_alloc {};
+  }
+  return p;
+}
+void operator delete( void* p ) noexcept { std::free( p ); }
+void operator delete( void* p, std::size_t ) noexcept { std::free( p ); }
+
+int main()
+{
+  int failed = 0;
+  for ( int op = 0; op < 5; op++ ) {
+    for ( long n = 0; n < 12; n++ ) {
+      glint::PageBook book { 40, 4 };
+      book.extend( 1, 30 );
+      book.extend( 2, 9 );
+      book.fork( 2, 3 );
+      book.release( 1 );
+      const auto line2 = book.context( 2 )->pages, line3 = book.context( 3 )->pages;
+      const auto free = book.free();
+      left = n;
+      bool threw = false;
+      try {
+        switch ( op ) {
+          case 0: book.extend( 9, 20 ); break;
+          case 1: book.extend( 3, 60 ); break;
+          case 2: book.fork( 2, 9 ); break;
+          case 3: book.compact(); break;
+          default: book.release( 3 ); break;
+        }
+      } catch ( const std::bad_alloc& ) {
+        threw = true;
+      }
+      left = -1;
+      failed += threw;
+      if ( threw && ( book.free() != free || book.context( 9 ) || book.context( 2 )->pages != line2 || book.context( 3 )->pages != line3 || op == 4 ) ) {
+        std::printf( "op %d, allocation %ld\n", op, n );
+        return 1;
+      }
+      book.release( 2 );
+      book.release( 3 );
+      book.release( 9 );
+      if ( book.free() != 40 || !book.extend( 1, 160 ) || book.free() != 0 ) {
+        std::printf( "op %d, allocation %ld: pages lost\n", op, n );
+        return 1;
+      }
+    }
+  }
+  return failed >= 8 ? 0 : 2;
+}
+"""
+
+
+def test_calls_that_memory_runs_out_in_change_nothing(tmp_path):
+    source, exe = tmp_path / "failing.cc", tmp_path / "failing"
+    source.write_text(FAILING)
+    host = os.path.join(os.path.dirname(os.path.abspath(glinthawk_amd.__file__)), "host")
+    subprocess.run(["g++", "-std=c++20", "-O1", "-Wall", "-Werror", "-I" + host, str(source), "-o", str(exe)], check=True, timeout=120)
+    ran = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert ran.returncode == 0, ran.stdout

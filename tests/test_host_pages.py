@@ -133,6 +133,9 @@ def test_tensors_that_are_refused():
         ops.copy_pages(pool, torch.zeros((2, 2), dtype=torch.int64))
     with pytest.raises(ValueError):
         ops.copy_pages(pool[:, ::2], [(0, 1)])
+    for pairs in ([(0, 2 ** 32 + 1)], [(0, -1)], [(0, pool.shape[0])], [(0, 1, 2), (3, 0, 1)]):
+        with pytest.raises(ValueError):
+            ops.copy_pages(pool, pairs)
     for logits, tokens in ((torch.zeros(2, 9), lengths.long()), (torch.zeros(2, 9), lengths[:1]), (torch.zeros(9, 2).t(), lengths), (torch.zeros(9), lengths)):
         with pytest.raises(ValueError):
             ops.token_logprobs(logits, tokens, 1, torch.zeros(16, dtype=torch.uint8))
