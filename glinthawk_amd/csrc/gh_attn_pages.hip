@@ -139,9 +139,9 @@ struct alignas( 4 * sizeof( T ) ) Piece
 //   packed: 64 columns a work-group, 16 a wave, stages of 32 keys that all four waves go through
 //   decode: 16 columns, stages of 64 keys, 16 a wave, the four joined through LDS at the end
 // The next stage's rows are asked for before a stage is computed.
-// Taken where rows cannot go straight to LDS in pieces of 16 bytes: head sizes that are no multiple of them, pages below 16 tokens, pool or rows that are not aligned, and
-// fp32 heads above 128.  Bound by its own conversions and LDS traffic: decode of 64 contexts of 2000 keys, 8 heads of 256 in f16, took it 1080 us (1.0 TB/s; the
-// streaming kernel 160), a prompt of 2048 tokens with those heads 1508 us (106).
+// Taken where rows cannot go straight to LDS in pieces of 16 bytes: head sizes that are no multiple of them, pages below 16 tokens, pool or rows that are not aligned.
+// Bound by its own conversions and LDS traffic.  f16, 8 heads on 4 kv heads of 36: decode of 64 contexts of 100 to 4000 keys 94 us (0.8 TB/s; heads of 40 in the streaming
+// kernel 45), a prompt of 4000 tokens 391 us (54).
 // =================================================================================================
 template<typename T, int NB, bool DECODE>
 __global__ __launch_bounds__( 256 ) void attn_pages_f32_kernel( const T* __restrict__ q, T* __restrict__ out, Call a )
@@ -406,6 +406,7 @@ __global__ __launch_bounds__( 256 ) void attn_pages_f32_kernel( const T* __restr
 // 16-byte chunks of a row are swizzled by the row (in the address a lane fetches) so that both reads touch every bank once.
 // The weights are rounded to the storage type for the second product, as the matrix units take them; the sum takes them rounded too.
 // fp32: both products 16 x 16 x 4, a chunk of K being four of its steps, weights as they are, and V read value by value; 16 keys a stage above 64 elements.
+// (64 contexts of 100 to 4000 keys, 8 heads of 256 in fp32: 357 us, 6.0 TB/s; in the tile kernel above 1530.)
 // W waves of a work-group take the stages of one run in turns and are joined through LDS.
 // f16, 8 kv heads of 128 with 8 queries each: 64 contexts of 57 to 4096 keys 90 us (6.0 TB/s), 1 of 301 keys 7.0 us, of which a launch that only stores takes 3;
 // bf16, 32 heads, 3 contexts of 20011 to 32768 keys: 226 us (5.7 TB/s), the launch that joins the splits (4.8) among them.
@@ -459,7 +460,7 @@ __device__ __forceinline__ void store4( E* to, float a, float b, float c, float 
 }
 
 template<uint32_t FIRST, typename Chunk>
-__device__ __forceinline__ void read_chunks( const uint32_t* at, Chunk ( &k )[8] )
+__device__ __forceinline__ void read_chunks( const uint32_t* at, Chunk* k )
 {
   asm volatile( "ds_read_b128 %0, %8 offset:%16\n\t"
                 "ds_read_b128 %1, %9 offset:%16\n\t"
@@ -480,7 +481,12 @@ __device__ __forceinline__ void read_chunks( const uint32_t* at, Chunk ( &k )[8]
 template<int CH, uint32_t FIRST, uint32_t SECOND, typename Chunk, uint32_t NU>
 __device__ __forceinline__ void read_keys( const uint32_t* at, Chunk ( &k )[NU][CH / 4] )
 {
-  if constexpr ( CH == 32 ) {
+  if constexpr ( CH == 64 ) {
+    static_assert( NU == 1, "" );
+    asm volatile( "s_waitcnt vmcnt(32)" ::: "memory" );
+    read_chunks<FIRST>( at, k[0] );
+    read_chunks<FIRST>( at + 8, k[0] + 8 );
+  } else if constexpr ( CH == 32 ) {
     if constexpr ( NU == 1 ) {
       asm volatile( "s_waitcnt vmcnt(16)" ::: "memory" );
     } else {
@@ -632,7 +638,7 @@ __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restri
 {
   constexpr bool F32 = sizeof( E ) == 4;
   constexpr uint32_t PER = 16 / sizeof( E );                    // elements of a chunk
-  constexpr uint32_t KEYS = F32 && CH == 32 ? 16 : 32;          // of a stage
+  constexpr uint32_t KEYS = F32 && CH >= 32 ? 16 : 32;          // of a stage
   constexpr uint32_t KK = CH / 4, NB = CH * PER / 16;           // chunks of a key that a lane reads, blocks of 16 dims
   constexpr uint32_t NU = KEYS / 16;
   constexpr uint32_t RPI = 64 / CH;            // rows that a load of the wave fetches
@@ -1396,21 +1402,21 @@ __global__ __launch_bounds__( 256, CH == 32 ? 1 : 2 ) void attn_pages_packed_ker
 // =================================================================================================
 // packed prompts in fp32, heads of up to CH chunks of 16 bytes: 16 CG columns a work-group of two times CG waves, 16 a wave
 //
-// Bound by the fp32 matrix instruction (16 x 16, 4 deep) where sequences are long.  Stages of 1024 / CH keys, two of them in LDS: K and V rows go there straight from
+// Bound by the fp32 matrix instruction (16 x 16, 4 deep) where sequences are long.  Stages of 1024 / CH keys (32 at least), two of them in LDS: K and V rows go there straight from
 // memory, the next stage's while one is computed, one barrier a stage; rows behind the last key and chunks behind a smaller head arrive as zeros.
 // The first CG waves take the first half of every stage's keys, the others the second half for the same columns, and are joined through LDS at the end: the longest
 // block of a launch is what a launch of few waits for.
 //   S^T = K Q^T     a 16-byte chunk of a key is four steps of the instruction; the scores of a lane: keys 4 g + i of column c
 //   O^T += V^T P^T  the weights are the second operand as they lie, V is read value by value: dim c of a block, of keys 4 g + i
 // Chunks are swizzled by the row so that both reads touch every bank once.
-// 5 prompts of 100 to 900 tokens, 12 heads of 64: 36 us, 70 TFLOP/s.
+// 5 prompts of 100 to 900 tokens, 12 heads of 64: 36 us, 70 TFLOP/s; one of 4000, 8 heads of 256: 712 us, 92 TFLOP/s (in the tile kernel above 1992).
 // =================================================================================================
 template<int CH, int CG>
 __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, float* __restrict__ out, const Call& a )
 {
-  constexpr uint32_t KEYS = 1024 / CH, TILES = KEYS / 32, RPI = 64 / CH, KK = CH / 4, NB = CH / 4;
-  constexpr uint32_t LOADS = 8 / CG; // of a wave for a stage's K, and for its V
-  __shared__ mfma_f32x4 s_k0[1024], s_k1[1024], s_v0[1024], s_v1[1024];
+  constexpr uint32_t KEYS = CH == 64 ? 32 : 1024 / CH, TILES = KEYS / 32, RPI = 64 / CH, KK = CH / 4, NB = CH / 4;
+  constexpr uint32_t LOADS = KEYS / RPI / ( 2 * CG ); // of a wave for a stage's K, and for its V
+  __shared__ mfma_f32x4 s_k0[KEYS * CH], s_k1[KEYS * CH], s_v0[KEYS * CH], s_v1[KEYS * CH];
 
   const uint32_t loader = __builtin_amdgcn_readfirstlane( threadIdx.x >> 6 ), wave = loader % CG, part = loader / CG, lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
   uint32_t number, h;
@@ -1618,7 +1624,7 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
 }
 
 template<int CH, int CG>
-__global__ __launch_bounds__( 128 * CG, CG ) void attn_pages_packed_f32_kernel( const float* __restrict__ q, float* __restrict__ out, Call a )
+__global__ __launch_bounds__( 128 * CG, CH == 64 ? CG / 2 : CG ) void attn_pages_packed_f32_kernel( const float* __restrict__ q, float* __restrict__ out, Call a )
 {
   packed_run_f32<CH, CG>( q, out, a );
 }
@@ -1726,7 +1732,7 @@ struct Plan
 };
 
 // The kernels that stream to LDS take heads made of 16-byte chunks, runs of 16 keys in one page, and everything aligned to 16 bytes.
-bool takes_tiles( const gh_shape* s, gh_dtype dt ) { return s->head_size * dtype_size( dt ) % 16 == 0 && s->head_size <= ( dt == GH_F32 ? 128 : 256 ); }
+bool takes_tiles( const gh_shape* s, gh_dtype dt ) { return s->head_size * dtype_size( dt ) % 16 == 0; }
 
 constexpr uint64_t MOST_PARTS = 65536; // of (query row, head, split) that leave partial results
 
@@ -1745,7 +1751,7 @@ Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, c
   const uint64_t blocks = decode ? batch * p.n_blocks : blocks_of();
   p.blocks = (uint32_t)blocks;
   if ( decode && tiles ) {
-    // Microseconds as measured on MI355X.  A stage of 16 KB takes a wave on its own 0.75, the four waves of a work-group 1.5, and 2.4 where the waves that fit
+    // Microseconds as measured on MI355X.  A stage of 16 KB takes a wave on its own 0.75, the four waves of a work-group 1.5 (fp32 heads above 128: 2.2, the matrix instructions of their 16 keys), and 2.4 where the waves that fit
     // (four a CU, eight of 16-bit heads up to 64) share the memory's rate; a round of work-groups takes 2 to begin and end; a split adds a launch (4) and 8 bytes an element
     // that go out and come back at 3 TB/s.  Where lengths differ the launch ends on the longest runs: a tenth of a wave's stages.
     // Measured, GQA heads (8 of 8 queries) in f16, us: 1 context of 301 keys, 4 waves 7.0, splits of 64 8.8 | 1 x 4096, 4 waves unsplit 39, splits of 64 10.8 |
@@ -1763,7 +1769,7 @@ Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, c
           continue;
         }
         const double stages = (double)( ( std::min( chunk, max_keys ) + stage * waves - 1 ) / ( stage * waves ) ), load = (double)( streams * splits * waves ) / slots;
-        const double alone = waves == 1 ? 0.75 : 1.5, full = std::max( alone, 2.4 * std::min( 1.0, load ) );
+        const double alone = dt == GH_F32 && wide ? 2.2 : waves == 1 ? 0.75 : 1.5, full = std::max( alone, 2.4 * std::min( 1.0, load ) );
         double us = stages * std::max( alone, 2.4 * load ) + 0.1 * stages * full + 2.0 * std::max( 1.0, load );
         if ( splits > 1 ) {
           us += 4.0 + (double)( rows * s->n_heads * splits ) * s->head_size * 8 / 3e6;
@@ -1836,7 +1842,7 @@ void launch_decode_tiles( const Plan& p, const Call& a, const void* q, void* out
   const E* tq = static_cast<const E*>( q );
   E* to = static_cast<E*>( out );
   if constexpr ( sizeof( E ) == 4 ) {
-    if ( a.gqa == 1 ) {
+    if ( a.gqa == 1 && a.size <= 128 ) {
       const dim3 grid( p.blocks * a.n_kv_heads, p.splits );
       if ( a.size <= 64 ) {
         p.waves > 1 ? attn_pages_decode_one_kernel<16, 4><<<grid, 256, 0, st>>>( tq, to, a ) : attn_pages_decode_one_kernel<16, 1><<<grid, 64, 0, st>>>( tq, to, a );
@@ -1867,11 +1873,11 @@ void launch_decode_tiles( const Plan& p, const Call& a, const void* q, void* out
     sizes( std::integral_constant<int, NARROW> {} );
   } else if ( a.size <= 128 ) {
     sizes( std::integral_constant<int, 2 * NARROW> {} );
-  } else if constexpr ( sizeof( E ) == 2 ) { // 64 KB of LDS a wave
+  } else { // 64 KB of LDS a wave
     if ( p.waves > 1 ) {
-      go( std::integral_constant<int, 32> {}, two, one );
+      go( std::integral_constant<int, 4 * NARROW> {}, two, one );
     } else {
-      go( std::integral_constant<int, 32> {}, one, one );
+      go( std::integral_constant<int, 4 * NARROW> {}, one, one );
     }
   }
 }
@@ -1885,8 +1891,10 @@ void launch_packed_tiles( const Plan& p, const Call& a, const void* q, void* out
     float* to = static_cast<float*>( out );
     if ( a.size <= 64 ) {
       p.waves == 8 ? attn_pages_packed_f32_kernel<16, 4><<<grid, 512, 0, st>>>( tq, to, a ) : attn_pages_packed_f32_kernel<16, 2><<<grid, 256, 0, st>>>( tq, to, a );
-    } else {
+    } else if ( a.size <= 128 ) {
       p.waves == 8 ? attn_pages_packed_f32_kernel<32, 4><<<grid, 512, 0, st>>>( tq, to, a ) : attn_pages_packed_f32_kernel<32, 2><<<grid, 256, 0, st>>>( tq, to, a );
+    } else {
+      p.waves == 8 ? attn_pages_packed_f32_kernel<64, 4><<<grid, 512, 0, st>>>( tq, to, a ) : attn_pages_packed_f32_kernel<64, 2><<<grid, 256, 0, st>>>( tq, to, a );
     }
   } else if ( a.size <= 64 ) {
     attn_pages_packed_kernel<E, 8><<<grid, 256, 0, st>>>( static_cast<const E*>( q ), static_cast<E*>( out ), a );
