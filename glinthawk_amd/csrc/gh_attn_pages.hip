@@ -557,8 +557,8 @@ __device__ __forceinline__ void read_rows( uint32_t at, mfma_f32x4 ( &v )[8] )
                 "ds_read_b128 %7, %8 offset:%16\n\t"
                 "s_waitcnt lgkmcnt(0)"
                 : "=&v"( v[0] ), "=&v"( v[1] ), "=&v"( v[2] ), "=&v"( v[3] ), "=&v"( v[4] ), "=&v"( v[5] ), "=&v"( v[6] ), "=&v"( v[7] )
-                : "v"( at ), "n"( FIRST ), "n"( FIRST + 1024 ), "n"( FIRST + 2048 ), "n"( FIRST + 3072 ), "n"( FIRST + 4096 ), "n"( FIRST + 5120 ), "n"( FIRST + 6144 ),
-                  "n"( FIRST + 7168 )
+                : "v"( at ), "n"( FIRST ), "n"( FIRST + 1 * 1024 ), "n"( FIRST + 2 * 1024 ), "n"( FIRST + 3 * 1024 ), "n"( FIRST + 4 * 1024 ), "n"( FIRST + 5 * 1024 ), "n"( FIRST + 6 * 1024 ),
+                  "n"( FIRST + 7 * 1024 )
                 : "memory" );
 }
 

@@ -142,7 +142,7 @@ __device__ __forceinline__ void finish_row( const Outputs& o, uint64_t row, Sums
 
 // grid: (parts, rows); a part: `per_part` columns, at most THREADS * PIECES * V.  One part: the row is finished here, else parts go to `sums`, `tops`.
 template<typename T, int THREADS, int PIECES>
-__global__ __launch_bounds__( THREADS, THREADS >= 512 ? ( THREADS == 512 || PIECES * 16 / sizeof( T ) <= 32 ? 8 : 4 ) : 4 ) void logprob_kernel( Outputs o, const T* __restrict__ logits, uint64_t row_stride, const uint32_t* __restrict__ tokens, uint32_t vocab,
+__global__ __launch_bounds__( THREADS, THREADS == 512 || ( THREADS == 1024 && PIECES * 16 / sizeof( T ) <= 32 ) ? 8 : 4 ) void logprob_kernel( Outputs o, const T* __restrict__ logits, uint64_t row_stride, const uint32_t* __restrict__ tokens, uint32_t vocab,
                                                             uint32_t n_top, uint32_t per_part, Sums* __restrict__ sums, uint64_t* __restrict__ tops )
 {
   constexpr int V = 16 / sizeof( T ), WAVES = THREADS / WAVE;
@@ -404,13 +404,17 @@ void launch_logprobs( const LogprobPlan& p, const Outputs& o, const void* logits
     go( few, std::integral_constant<int, 4> {} );
   } else if ( pieces <= 2048 ) {
     go( many, std::integral_constant<int, 2> {} );
-  } else if ( pieces <= 4096 && std::is_same_v<T, __half> && rows >= 512 ) {
-    // more work-groups a CU, whose short phases fill each other's gaps (2047 rows of 32000, 20 alternatives: 40 us, with 1024 threads 46, with 256 43; 256 rows: 11.0 and 10.2; bf16 does not
-    // fit the registers so: 47 and 47)
-    go( std::integral_constant<int, 512> {}, std::integral_constant<int, 8> {} );
   } else if ( pieces <= 4096 ) {
+    // f16: more work-groups a CU, whose short phases fill each other's gaps (2047 rows of 32000, 20 alternatives: 40 us, with 1024 threads 46, with 256 43; 256 rows: 11.0 and
+    // 10.2; bf16 does not fit the registers so: 47 and 47)
+    if constexpr ( std::is_same_v<T, __half> ) {
+      if ( rows >= 512 ) {
+        go( std::integral_constant<int, 512> {}, std::integral_constant<int, 8> {} );
+        return;
+      }
+    }
     go( many, std::integral_constant<int, 4> {} );
-  } else {
+  } else if constexpr ( sizeof( T ) == 4 ) { // (a part has up to 32768 columns)
     go( many, std::integral_constant<int, 8> {} );
   }
 }
