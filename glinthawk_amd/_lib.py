@@ -187,6 +187,7 @@ SIGNATURES = {
     "gh_copy_pages_host": (_i, [_vp, _u64, _u64, _u32, _u64, _u64, _vp, _u64, _vp]),
     "gh_token_logprobs_workspace": (_u64, [_u64, _u64, _u32]),
     "gh_token_logprobs": (_i, [_vp, _vp, _vp, _vp, _vp, _u64, _vp, _u64, _u64, _u32, _i, _vp, _u64, _vp]),
+    "gh_token_logprobs_fill": (_i, [_vp, _f, _vp, _vp, _vp, _vp, _u64, _vp, _u64, _u64, _u32, _i, _vp, _u64, _vp]),
     "gh_embed_step": (_i, [_vp, _vp, _vp, _u64, _u64, _u64, _u64, _u32, _vp, _vp, _u64, _u64, _u64, _vp, _u64, _step, _i, _vp]),
     "gh_matmul_scaled_argmax": (_i, [_vp, _vp, _vp, _vp, _u64, _u64, _u64, _f, _i, _vp]),
     "gh_embed_positions": (_i, [_vp, _vp, _vp, _u64, _u32, _vp, _vp, _u64, _u64, _u64, _vp, _u64, _i, _vp]),

@@ -30,6 +30,8 @@ struct Outputs
   float* entropy;
   uint32_t* top_ids;
   float* top_logprobs;
+  bool fills; // logprob of a token that is none: `fill`, or left as it is
+  float fill;
 };
 
 // ---- numbers in the order of the values --------------------------------------------------------
@@ -132,8 +134,12 @@ __device__ __forceinline__ void finish_row( const Outputs& o, uint64_t row, Sums
 {
   const float m = z.m == -INFINITY ? 0.0f : z.m;
   const float log_s = logf( z.s );
-  if ( o.logprob != nullptr && tokens[row] < vocab ) {
-    o.logprob[row] = z.m == -INFINITY ? __builtin_nanf( "" ) : ( given - m ) - log_s;
+  if ( o.logprob != nullptr ) {
+    if ( tokens[row] < vocab ) {
+      o.logprob[row] = z.m == -INFINITY ? __builtin_nanf( "" ) : ( given - m ) - log_s;
+    } else if ( o.fills ) {
+      o.logprob[row] = o.fill;
+    }
   }
   if ( o.entropy != nullptr ) {
     o.entropy[row] = log_s - z.t / z.s;
@@ -419,25 +425,17 @@ void launch_logprobs( const LogprobPlan& p, const Outputs& o, const void* logits
   }
 }
 
-} // namespace
-} // namespace gh
-
-using namespace gh;
-
-extern "C" {
-
-uint64_t gh_token_logprobs_workspace( uint64_t rows, uint64_t vocab, uint32_t n_top ) { return rows == 0 || vocab == 0 ? 0 : plan_logprobs( rows, vocab, n_top ).bytes; }
-
-int gh_token_logprobs( float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs, const void* logits, uint64_t row_stride, const uint32_t* tokens_dev,
-                       uint64_t vocab, uint64_t rows, uint32_t n_top, gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream )
+// Both entry points
+int token_logprobs( const char* op, const Outputs& o, const void* logits, uint64_t row_stride, const uint32_t* tokens_dev, uint64_t vocab, uint64_t rows, uint32_t n_top,
+                    gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream )
 {
   if ( rows != 0 ) { // what can be said without a device is said first
-    GH_REQUIRE( logits && ( logprob == nullptr || tokens_dev ) && ( n_top == 0 || ( top_ids && top_logprobs ) ), "gh_token_logprobs: NULL pointer" );
-    GH_REQUIRE( dt == GH_F16 || dt == GH_F32 || dt == GH_BF16, "gh_token_logprobs: unsupported dtype %d", (int)dt );
-    GH_REQUIRE( vocab > 0 && vocab <= 1u << 21 && rows <= 65535, "gh_token_logprobs: bad shape (up to 65535 rows of up to 2097152 values)" );
-    GH_REQUIRE( n_top <= MAX_TOP && n_top <= vocab, "gh_token_logprobs: %u alternatives of %llu values (at most %u)", n_top, (unsigned long long)vocab, MAX_TOP );
-    GH_REQUIRE( row_stride >= vocab || rows == 1, "gh_token_logprobs: rows of %llu values lie %llu apart", (unsigned long long)vocab, (unsigned long long)row_stride );
-    GH_REQUIRE( reinterpret_cast<uintptr_t>( logits ) % dtype_size( dt ) == 0, "gh_token_logprobs: logits are not aligned to their elements" );
+    GH_REQUIRE( logits && ( o.logprob == nullptr || tokens_dev ) && ( n_top == 0 || ( o.top_ids && o.top_logprobs ) ), "%s: NULL pointer", op );
+    GH_REQUIRE( dt == GH_F16 || dt == GH_F32 || dt == GH_BF16, "%s: unsupported dtype %d", op, (int)dt );
+    GH_REQUIRE( vocab > 0 && vocab <= 1u << 21 && rows <= 65535, "%s: bad shape (up to 65535 rows of up to 2097152 values)", op );
+    GH_REQUIRE( n_top <= MAX_TOP && n_top <= vocab, "%s: %u alternatives of %llu values (at most %u)", op, n_top, (unsigned long long)vocab, MAX_TOP );
+    GH_REQUIRE( row_stride >= vocab || rows == 1, "%s: rows of %llu values lie %llu apart", op, (unsigned long long)vocab, (unsigned long long)row_stride );
+    GH_REQUIRE( reinterpret_cast<uintptr_t>( logits ) % dtype_size( dt ) == 0, "%s: logits are not aligned to their elements", op );
   }
   if ( int rc = ensure_init() ) {
     return rc;
@@ -446,13 +444,12 @@ int gh_token_logprobs( float* logprob, float* entropy, uint32_t* top_ids, float*
     return GH_OK;
   }
   const LogprobPlan p = plan_logprobs( rows, vocab, n_top );
-  GH_REQUIRE( p.bytes == 0 || ( workspace != nullptr && reinterpret_cast<uintptr_t>( workspace ) % 16 == 0 ), "gh_token_logprobs: a 16-byte aligned workspace is needed" );
+  GH_REQUIRE( p.bytes == 0 || ( workspace != nullptr && reinterpret_cast<uintptr_t>( workspace ) % 16 == 0 ), "%s: a 16-byte aligned workspace is needed", op );
   if ( p.bytes > workspace_bytes ) {
-    return fail( GH_ERR_WORKSPACE, "gh_token_logprobs: workspace of %llu bytes, %llu are needed", (unsigned long long)workspace_bytes, (unsigned long long)p.bytes );
+    return fail( GH_ERR_WORKSPACE, "%s: workspace of %llu bytes, %llu are needed", op, (unsigned long long)workspace_bytes, (unsigned long long)p.bytes );
   }
   uint64_t* tops = static_cast<uint64_t*>( workspace );
   Sums* sums = reinterpret_cast<Sums*>( tops + rows * p.parts * n_top );
-  const Outputs o { logprob, entropy, top_ids, top_logprobs };
   hipStream_t st = as_stream( stream );
   switch ( dt ) {
     case GH_F16: launch_logprobs<__half>( p, o, logits, row_stride, tokens_dev, (uint32_t)vocab, rows, n_top, sums, tops, st ); break;
@@ -465,6 +462,27 @@ int gh_token_logprobs( float* logprob, float* entropy, uint32_t* top_ids, float*
     GH_LAUNCH_CHECK();
   }
   return GH_OK;
+}
+
+} // namespace
+} // namespace gh
+
+using namespace gh;
+
+extern "C" {
+
+uint64_t gh_token_logprobs_workspace( uint64_t rows, uint64_t vocab, uint32_t n_top ) { return rows == 0 || vocab == 0 ? 0 : plan_logprobs( rows, vocab, n_top ).bytes; }
+
+int gh_token_logprobs( float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs, const void* logits, uint64_t row_stride, const uint32_t* tokens_dev,
+                       uint64_t vocab, uint64_t rows, uint32_t n_top, gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream )
+{
+  return token_logprobs( "gh_token_logprobs", { logprob, entropy, top_ids, top_logprobs, false, 0.0f }, logits, row_stride, tokens_dev, vocab, rows, n_top, dt, workspace, workspace_bytes, stream );
+}
+
+int gh_token_logprobs_fill( float* logprob, float fill, float* entropy, uint32_t* top_ids, float* top_logprobs, const void* logits, uint64_t row_stride,
+                            const uint32_t* tokens_dev, uint64_t vocab, uint64_t rows, uint32_t n_top, gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream )
+{
+  return token_logprobs( "gh_token_logprobs_fill", { logprob, entropy, top_ids, top_logprobs, true, fill }, logits, row_stride, tokens_dev, vocab, rows, n_top, dt, workspace, workspace_bytes, stream );
 }
 
 } // extern "C"

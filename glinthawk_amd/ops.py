@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 from typing import Optional, Sequence
 
 import torch
@@ -541,7 +542,8 @@ def token_logprobs_workspace(rows: int, vocab: int, n_top: int) -> int:
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, n_top: int = 0, workspace: Optional[torch.Tensor] = None):
-    """(log probability of each row's token, entropy, (rows, n_top) indices of the largest values, their log probabilities)"""
+    """(log probability of each row's token, entropy, (rows, n_top) indices of the largest values, their log probabilities).  The log probability of a token that is
+    not below the vocabulary (-1 for padding, say) is NaN."""
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise ValueError("rows of logits lie with their values one behind the other")
     (rows, vocab), device = logits.shape, logits.device
@@ -554,8 +556,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, n_top: int = 0, w
     # (0.4 us less each than from sizes alone)
     ids = torch.empty_strided((rows, n_top), (n_top, 1), dtype=torch.int32, device=device)
     values = torch.empty_strided((rows, n_top), (n_top, 1), dtype=torch.float32, device=device)
-    check(lib().gh_token_logprobs(given.data_ptr(), entropy.data_ptr(), ids.data_ptr(), values.data_ptr(), logits.data_ptr(), logits.stride(0), tokens.data_ptr(), vocab, rows,
-                                  n_top, _dt(logits), workspace.data_ptr(), workspace.nbytes, _stream_on(device)), "gh_token_logprobs")
+    check(lib().gh_token_logprobs_fill(given.data_ptr(), math.nan, entropy.data_ptr(), ids.data_ptr(), values.data_ptr(), logits.data_ptr(), logits.stride(0), tokens.data_ptr(),
+                                       vocab, rows, n_top, _dt(logits), workspace.data_ptr(), workspace.nbytes, _stream_on(device)), "gh_token_logprobs_fill")
     return given, entropy, ids, values
 
 

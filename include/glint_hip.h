@@ -423,6 +423,9 @@ int gh_copy_pages_host( void* pool, uint64_t page_stride, uint64_t page_bytes, u
 uint64_t gh_token_logprobs_workspace( uint64_t rows, uint64_t vocab, uint32_t n_top );
 int gh_token_logprobs( float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs, const void* logits, uint64_t row_stride, const uint32_t* tokens_dev,
                        uint64_t vocab, uint64_t rows, uint32_t n_top, gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream );
+/* The same, with logprob(i) = fill where the token is not below vocab (padding, say): every value of logprob is written. */
+int gh_token_logprobs_fill( float* logprob, float fill, float* entropy, uint32_t* top_ids, float* top_logprobs, const void* logits, uint64_t row_stride,
+                            const uint32_t* tokens_dev, uint64_t vocab, uint64_t rows, uint32_t n_top, gh_dtype dt, void* workspace, uint64_t workspace_bytes, gh_stream stream );
 
 /* ---- designs whose sizes come at run time ---------------------------------------------------------
  * Ops of decoder-only designs beyond Llama2 (no counterpart in the reference): storage type GH_BF16 or GH_F32, the residual stream x,
