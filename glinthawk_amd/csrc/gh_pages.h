@@ -64,8 +64,8 @@ struct Packed
     const uint32_t b = begin( i ), e = begin( i + 1 );
     return e > b ? e - b : 0;
   }
-  // position of its first token, so that sums of it and a number of tokens stay below 2^32
-  __device__ __forceinline__ uint32_t begin_pos( uint32_t i ) const { return start ? min( start[i], 0x3fffffffu ) : 0u; }
+  // position of its first token, so that sums of it and a number of tokens (at most 2^24) stay below 2^32; a table reaches no position beyond
+  __device__ __forceinline__ uint32_t begin_pos( uint32_t i ) const { return start ? min( start[i], 0x7fffffffu ) : 0u; }
 };
 
 // sum or maximum over the wave, in every lane: rows of 16 lanes by DPP, the four rows by lane reads
