@@ -123,11 +123,13 @@ __device__ __forceinline__ Sums join( Sums a, Sums b )
   return r;
 }
 
-// S and T from sums over 2^d and 2^d d with d = x log2(e) - c: c is m log2(e) but for its rounding, which is taken out here
+// S and T from sums over 2^d and 2^d d with d = x log2(e) - c: c is m log2(e) but for its rounding, which is taken out here.  The largest value's own weight is what
+// the sum is divided by, so that S is 1 at least (no log probability above 0), and T is no more than 0 (no entropy below 0).
 __device__ __forceinline__ Sums sums_of( float max_m, float m, float c, float s, float t )
 {
   const float off = __builtin_fmaf( m, LOG2E, -c ); // x log2(e) - c = (x - m) log2(e) + off
-  return { max_m, s * __builtin_amdgcn_exp2f( -off ), __builtin_amdgcn_exp2f( -off ) * ( __builtin_fmaf( -off, s, t ) * 0.693147180559945309417f ) };
+  const float w = __builtin_amdgcn_exp2f( off ), below = __builtin_fmaf( -off, s, t );
+  return { max_m, s / w, ( below > 0.0f ? 0.0f : below ) / w * 0.693147180559945309417f };
 }
 
 __device__ __forceinline__ void finish_row( const Outputs& o, uint64_t row, Sums z, const uint32_t* tokens, uint32_t vocab, float given )
@@ -254,6 +256,10 @@ __global__ __launch_bounds__( THREADS, THREADS == 512 || ( THREADS == 1024 && PI
     }
   }
   __syncthreads();
+  const uint32_t count = s_count;
+  if ( count <= CANDIDATES && threadIdx.x >= max( max( count, n_top ), 1u ) ) {
+    return; // nothing to rank or to write, and no use for the row's sums
+  }
   float2 total = s_sums[0];
 #pragma unroll
   for ( int w = 1; w < WAVES; w++ ) {
@@ -281,7 +287,6 @@ __global__ __launch_bounds__( THREADS, THREADS == 512 || ( THREADS == 1024 && PI
       o.top_logprobs[row * n_top + rank] = ( value_of( number ) - m ) - log_s;
     }
   };
-  const uint32_t count = s_count;
   if ( count <= CANDIDATES ) {
     for ( uint32_t i = threadIdx.x; i < count; i += THREADS ) {
       const uint64_t number = s_number[i];

@@ -1,4 +1,4 @@
-"""Log probabilities at the edges of what the call takes: tokens that are none."""
+"""Log probabilities at the edges of what the call takes: tokens that are none, rows with one value."""
 import pytest
 import torch
 
@@ -7,6 +7,7 @@ from pages_plain import STEP32, logprobs
 
 pytestmark = pytest.mark.gpu
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+INF = float("inf")
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -42,3 +43,24 @@ def test_the_value_for_tokens_that_are_none():
     want = logprobs(logits, tokens.clamp(0, 99), 1)[0]
     assert given[1] == -2.5 and given[2] == -2.5
     assert float((given.double() - want)[[0, 3]].abs().max()) <= 32 * STEP32 * 8
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("vocab,values", [(40, 60000), (5000, 3000), (40000, 1000)])
+def test_one_finite_value_has_the_whole_weight(vocab, values, dtype):
+    """A constrained step that leaves one token: its log probability is 0, not above, and the entropy 0, not below (f16: powers of 2 relative to a rounded point within
+    2^-16 (300 log2(e) < 2^9), one product with it off by its last place, 2^-24 of it)."""
+    x = torch.full((values, vocab), -INF, dtype=dtype, device="cuda")
+    x[:, 3] = torch.linspace(-300, 300, values).to(dtype).cuda()
+    given, entropy, ids, top = ops.token_logprobs(x, torch.full((values,), 3, dtype=torch.int32, device="cuda"), 1)
+    assert bool((given == 0).all()) and bool((entropy >= 0).all()) and float(entropy.max()) <= (2.0 ** -40 if dtype == F16 else 0) and bool((top == 0).all()) and bool((ids == 3).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_log_probabilities_are_never_above_zero(dtype):
+    """One value far above the others, whose weights do not reach the sum's last place."""
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn((4000, 900), generator=g).to(dtype).cuda()
+    x[:, 5] = torch.linspace(15, 60, 4000).to(dtype).cuda()
+    given, entropy, _, top = ops.token_logprobs(x, torch.full((4000,), 5, dtype=torch.int32, device="cuda"), 2)
+    assert bool((given <= 0).all()) and bool((top <= 0).all()) and bool((entropy >= 0).all())
