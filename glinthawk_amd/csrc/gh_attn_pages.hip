@@ -417,7 +417,11 @@ typedef short v4s __attribute__( ( ext_vector_type( 4 ) ) );
 typedef short v8s __attribute__( ( ext_vector_type( 8 ) ) );
 typedef __attribute__( ( address_space( 3 ) ) ) v4s* lds_v4s;
 
-constexpr float LAZY = 8.0f; // the reference point of the exponentials stays until a maximum is 2^LAZY above it: weights up to 256, fewer rescalings
+constexpr float LAZY = 8.0f; // the reference point of the exponentials stays until a maximum is 2^LAZY above it: fewer rescalings
+// The reference point lies so many powers of two below the maximum it was taken from.  f16 weights then go up to 2^15, and what rounds to 0 is below 2^-32 of the largest
+// (at 0 it would be 2^-25, and the weights of a long context next to one key far above it would be lost).
+template<typename E>
+constexpr float LIFT = std::is_same_v<E, __half> ? 7.0f : 0.0f;
 
 // maximum over the lanes that share a column, 16 lanes apart, without a trip through LDS
 [[maybe_unused]] __device__ __forceinline__ float column_max( float v )
@@ -784,7 +788,7 @@ __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restri
         acc[n] *= alpha;
       }
     }
-    const float ms = m == -INFINITY ? 0.0f : m;
+    const float ms = m == -INFINITY ? 0.0f : m - LIFT<E>;
     float p[4 * NU], sum[2] = { 0, 0 };
 #pragma unroll
     for ( uint32_t e = 0; e < 4 * NU; e++ ) {
@@ -883,7 +887,7 @@ __device__ __forceinline__ void decode_run( const E* __restrict__ q, E* __restri
     }
   }
   if ( a.splits > 1 && g4 == 0 ) {
-    a.part_ml[slot * 2] = m;
+    a.part_ml[slot * 2] = m - LIFT<E>;
     a.part_ml[slot * 2 + 1] = l;
   }
 }
@@ -1290,7 +1294,7 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
         }
       }
     }
-    const float ms = m == -INFINITY ? 0.0f : m;
+    const float ms = m == -INFINITY ? 0.0f : m - LIFT<E>;
     // weights of keys 16 kk .. 16 kk + 15, packed as the second operand of their steps
     typedef uint32_t u32x4 __attribute__( ( ext_vector_type( 4 ) ) );
     u32x4 pk[4];
@@ -1368,7 +1372,7 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
         }
       }
       if ( g2 == 0 ) {
-        a.part_ml[slot * 2] = m;
+        a.part_ml[slot * 2] = m - LIFT<E>;
         a.part_ml[slot * 2 + 1] = l;
       }
     } else {

@@ -1,12 +1,13 @@
-"""Attention over a cache in pages at the edges of what the calls take: far positions."""
+"""Attention over a cache in pages at the edges of what the calls take: far positions, weights far below the largest."""
 import pytest
 import torch
 
 from glinthawk_amd import Shape, ops
-from pages_plain import HALF_STEP, STEP32
+from pages_plain import HALF_STEP, STEP32, Pool, attention, hold
 
 pytestmark = pytest.mark.gpu
-F16, F32 = torch.float16, torch.float32
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+INF = float("inf")
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -46,3 +47,75 @@ def test_a_prompt_behind_more_than_2_30_keys(start, dtype):
     assert shared or bool((pool[0] == 0).all())
     want = torch.tensor([1.0, 2.0, 2.0], device="cuda")[:, None].expand(3, size)
     assert float((xb.float() - want).abs().max()) <= 2 * (2 ** 30 * 2.718281828 ** -40 + 64 * STEP32 * 40 + 2 * HALF_STEP[dtype])
+
+
+def sink(dtype, keys, size=128, kv_heads=1):
+    """A pool of one context whose key 0 lies 25.4 powers of two above all others, with values 0 there and 1 elsewhere; the queries' element, the exact result for n keys."""
+    pool = torch.zeros((-(-keys // 16), 16, 2 * kv_heads * size), dtype=dtype, device="cuda")
+    pool[:, :, kv_heads * size:] = 1.0
+    pool[0, 0, kv_heads * size:] = 0.0
+    pool[0, 0, 0:kv_heads * size:size] = 14.125          # the same in all types
+    x = 14.125
+    low = 2.718281828459045 ** (-x * x * size ** -0.5)
+    return pool, x, lambda n: (n - 1) * low / (1 + (n - 1) * low)
+
+
+def room_for(dtype, n, exact):
+    # weights: relative, or where they are small for the type half its least difference, 2^-25 of 2^7; sums of n terms; the result
+    return exact * (3 * HALF_STEP[dtype] + 2 * n * STEP32 + 64 * STEP32 * 26) + (n * 2.0 ** -32 + 2.0 ** -25 if dtype == F16 else 0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_one_key_far_above_a_long_context_decode(dtype):
+    keys, batch, heads = 40000, 1024, 64
+    pool, x, exact = sink(dtype, keys)
+    table = torch.arange(pool.shape[0], dtype=torch.int32, device="cuda").expand(batch, -1).contiguous()      # contexts that share all pages
+    q = torch.zeros((batch, heads, 128), dtype=dtype, device="cuda")
+    q[:, :, 0] = x
+    lengths = torch.full((batch,), keys, dtype=torch.int32, device="cuda")
+    lengths[0], lengths[1] = 30001, 100
+    xb = torch.zeros((batch, heads * 128), dtype=dtype, device="cuda")
+    ops.attn_decode_paged(q.reshape(batch, -1), ops.pages(pool, table), lengths, xb, keys, shape_of(heads, 1, 128))
+    for row, n in ((0, 30001), (1, 100), (2, keys), (batch - 1, keys)):
+        assert float((xb[row].double() - exact(n)).abs().max()) <= room_for(dtype, n, exact(n)), n
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("tokens", [3, 1024])
+def test_one_key_far_above_a_long_context_packed(tokens, dtype):
+    keys, heads, kv_heads = 40000, 16, 2
+    pool, x, exact = sink(dtype, keys, kv_heads=kv_heads)
+    table = torch.arange(pool.shape[0], dtype=torch.int32, device="cuda")[None].contiguous()
+    q = torch.zeros((tokens, heads, 128), dtype=dtype, device="cuda")
+    q[:, :, 0] = x
+    xb = torch.zeros((tokens, heads * 128), dtype=dtype, device="cuda")
+    start = keys - tokens
+    ops.attn_packed(q.reshape(tokens, -1), ops.pages(pool, table), ints(0, tokens), ints(start), xb, keys, shape_of(heads, kv_heads, 128))
+    for t in sorted({0, 1, tokens // 2, tokens - 1}):
+        n = start + t + 1
+        assert float((xb[t].double() - exact(n)).abs().max()) <= room_for(dtype, n, exact(n)), t
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,size", [(8, 1, 128), (4, 4, 64), (3, 1, 36), (2, 1, 200)])
+def test_packed_scores_of_every_size(heads, kv_heads, size, dtype):
+    """Scores far apart (one key has all the weight, others next to none), all equal, all at the type's lowest value, and an infinity where the formula gives NaN."""
+    tokens, start = 70, 600
+    pool = Pool([start + tokens], kv_heads, size, dtype)
+    q = torch.randn((tokens, heads * size), generator=torch.Generator().manual_seed(1)).to(dtype).cuda() * 30
+    q[20:30] = 0
+    q[30:40] = -torch.finfo(dtype).max if dtype == F16 else -3.0e4
+    q[40:50] = q[40:50] / 10
+
+    def run():
+        xb = torch.full_like(q, 7.0)
+        ops.attn_packed(q, ops.pages(pool.pool, pool.table), ints(0, tokens), ints(start), xb, start + tokens, shape_of(heads, kv_heads, size))
+        return xb.reshape(tokens, heads, size)
+
+    want, off = attention(q.reshape(tokens, heads, size), pool.k(0), pool.v(0), start, dtype, dtype != F32)
+    hold(run(), want, off)
+    q[60, 5] = INF
+    got = run()
+    assert bool(torch.isnan(got[60, 0]).all()) and bool(torch.isfinite(got[60, 1:]).all())
+    rest = [t for t in range(tokens) if t != 60]
+    hold(got[rest], want[rest], off[rest])
