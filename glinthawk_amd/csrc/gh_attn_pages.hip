@@ -100,27 +100,207 @@ __device__ __forceinline__ void number_and_head( const Call& a, uint32_t* number
 // keys that token t of a block's sequence attends
 __device__ __forceinline__ uint32_t visible( const Call& a, const Block& b, uint32_t t ) { return min( b.start + t + 1, a.max_keys ); }
 
-// A column (by its number in the sequence) of a tile kernel's split once more, by a whole wave, with its result put where the tile's would be.
+// sum over the lanes that share a column, 16 lanes apart
+__device__ __forceinline__ float column_sum( float v ) { return sum_rows( sum_halves( v, v ), sum_halves( v, v ) ); }
+
+// ---- what a masked key's row must not do ---------------------------------------------------------------
+// A tile multiplies the values of keys that a column does not attend by a weight of zero, and an infinity or a NaN among them makes a NaN of the sum.  Packed prompts'
+// kernels look for columns whose result holds a NaN or an infinity, but not in the sum of the weights (a NaN there is one of an attended key's score, and the whole row is
+// NaN).  Where all the values are finite that a column of the wave may have met without attending them, the result is the formula's (an infinite value whose weight is 0
+// as the tile has it gives NaN); else those columns are made again here, 16 at a time, by the wave alone and with exact masks.
+// 2048 tokens, 8 heads of 128 on one, f16, 53 us a call on its own: with a row of NaN 53 us; with NaN in the values alone of one of the first tokens 57, of one of the last
+// (whose wave walks all the keys before it) 580; with infinite values in every row 620.  4096 tokens of 64 heads: 300, 330, 385, 1380 and 3900.
+
+// whether the values of a head are finite in all rows [from, to), by a whole wave
 template<typename T>
-__device__ __noinline__ void walk_column( const T* q, T* out, Call a, Block b, uint32_t col, uint32_t k_begin, uint32_t k_end )
+__device__ __noinline__ bool finite_values( Pages p, uint32_t seq, uint32_t v_off, uint32_t size, uint32_t from, uint32_t to )
 {
   const uint32_t lane = threadIdx.x & 63;
-  const uint64_t place = (uint64_t)( b.row0 + col / a.gqa ) * a.n_kv_heads * a.gqa + b.h * a.gqa + col % a.gqa, slot = place * a.splits + b.split;
-  float m, l, acc[4];
-  walk_row<T>( q + place * a.size, a.pages, b.seq, b.h * a.size, ( a.n_kv_heads + b.h ) * a.size, a.size, k_begin, k_end, a.scale_log2e, &m, &l, acc );
-  for ( uint32_t u = 0; u < 4; u++ ) {
-    const uint32_t d = 64 * u + lane;
-    if ( d < a.size ) {
-      if ( a.splits == 1 ) {
-        out[place * a.size + d] = from_f32<T>( acc[u] / l );
-      } else {
-        a.part_out[slot * a.size + d] = acc[u];
+  float probe = 0.0f;
+  for ( uint32_t key = from; key < to; key++ ) {
+    const T* v = reinterpret_cast<const T*>( p.row( seq, key ) ) + v_off;
+    for ( uint32_t d = lane; d < size; d += 64 ) {
+      probe += 0.0f * to_f32( v[d] );
+    }
+  }
+  return __builtin_amdgcn_ballot_w64( probe != probe ) == 0;
+}
+
+// Four neighbouring values of a row of `size`, from d on, 0 behind it, without a branch (a load behind one would be waited for before the next).
+// FOURS: the size is a multiple of 4.
+template<typename T, bool FOURS>
+struct Four
+{
+  T e[4];
+  __device__ __forceinline__ void load( const T* row, uint32_t d, uint32_t size )
+  {
+    if constexpr ( FOURS ) {
+      __builtin_memcpy( e, row + ( d < size ? d : 0 ), sizeof( e ) ); // rows may begin anywhere
+    }
+#pragma unroll
+    for ( uint32_t i = 0; i < 4; i++ ) {
+      if constexpr ( !FOURS ) {
+        e[i] = row[min( d + i, size - 1 )];
+      }
+      e[i] = d + i < size ? e[i] : from_f32<T>( 0.0f );
+    }
+  }
+};
+
+// Columns col0 + c of block b, those with bit c of `which` set, over the keys of its split [k_begin, k_most): results put where the tile's are.
+// Keys that all of them see in tiles of 16, products in fp32 matrix instructions with operands straight from memory; the others one by one.
+template<typename T, int NB, bool FOURS>
+__device__ __forceinline__ void columns_again( const T* __restrict__ q, T* __restrict__ out, const Call& a, const Block& b, uint32_t col0, uint32_t which, uint32_t k_begin, uint32_t k_most )
+{
+  const uint32_t lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4, n_heads = a.n_kv_heads * a.gqa;
+  const bool ok = which >> c & 1;
+  auto end_of = [&]( uint32_t col ) { return min( visible( a, b, col / a.gqa ), k_most ); };
+  const uint32_t t_all = end_of( col0 + (uint32_t)__builtin_ctz( which ) ), t_end = end_of( col0 + 31 - (uint32_t)__builtin_clz( which ) );
+  const uint32_t col = ok ? col0 + c : col0 + (uint32_t)__builtin_ctz( which ), my_end = end_of( col );
+  const uint64_t place = (uint64_t)( b.row0 + col / a.gqa ) * n_heads + b.h * a.gqa + col % a.gqa;
+  const uint32_t k_off = b.h * a.size, v_off = ( a.n_kv_heads + b.h ) * a.size;
+  auto row = [&]( uint32_t key ) { return reinterpret_cast<const T*>( a.pages.row( b.seq, key ) ); };
+
+  mfma_f32x4 acc[NB]; // element i of acc[n]: dim 16 n + 4 g4 + i of the lane's column
+#pragma unroll
+  for ( int n = 0; n < NB; n++ ) {
+    acc[n] = mfma_f32x4 { 0, 0, 0, 0 };
+  }
+  float m = -INFINITY, l = 0.0f;
+  Four<T, FOURS> x[NB]; // of the query: dims 16 n + 4 g4 ..
+#pragma unroll
+  for ( int n = 0; n < NB; n++ ) {
+    x[n].load( q + place * a.size, 16 * n + 4 * g4, a.size );
+  }
+  uint32_t t0 = k_begin;
+  const T *k_row = row( t0 + min( c, t_end - 1 - t0 ) ), *v_row[4]; // (asked for a tile ahead)
+#pragma unroll
+  for ( uint32_t i = 0; i < 4; i++ ) {
+    v_row[i] = row( t0 + min( 4 * g4 + i, t_end - 1 - t0 ) );
+  }
+  for ( ; t0 + 16 <= t_all; t0 += 16 ) {
+    Four<T, FOURS> k[NB];
+    T v[NB][4];
+#pragma unroll
+    for ( int n = 0; n < NB; n++ ) {
+      k[n].load( k_row + k_off, 16 * n + 4 * g4, a.size );
+    }
+#pragma unroll
+    for ( uint32_t n = 0; n < NB; n++ ) {
+#pragma unroll
+      for ( int i = 0; i < 4; i++ ) {
+        v[n][i] = v_row[i][v_off + min( 16 * n + c, a.size - 1 )];
+        v[n][i] = 16 * n + c < a.size ? v[n][i] : from_f32<T>( 0.0f );
+      }
+    }
+    const uint32_t ahead = min( t0 + 16, t_end - 1 );
+    k_row = row( min( ahead + c, t_end - 1 ) );
+#pragma unroll
+    for ( uint32_t i = 0; i < 4; i++ ) {
+      v_row[i] = row( min( ahead + 4 * g4 + i, t_end - 1 ) );
+    }
+    mfma_f32x4 st = { 0, 0, 0, 0 };
+#pragma unroll
+    for ( int n = 0; n < NB; n++ ) {
+#pragma unroll
+      for ( int e = 0; e < 4; e++ ) {
+        st = __builtin_amdgcn_mfma_f32_16x16x4f32( to_f32( k[n].e[e] ), to_f32( x[n].e[e] ), st, 0, 0, 0 );
+      }
+    }
+    float mx = -INFINITY, p[4];
+#pragma unroll
+    for ( int i = 0; i < 4; i++ ) {
+      p[i] = st[i] * a.scale_log2e;
+      mx = fmaxf( mx, p[i] );
+    }
+    mx = fmaxf( mx, __shfl_xor( mx, 16, WAVE ) );
+    mx = fmaxf( mx, __shfl_xor( mx, 32, WAVE ) );
+    const float m_new = fmaxf( m, mx ), m_safe = m_new == -INFINITY ? 0.0f : m_new, alpha = fast_exp2( m - m_safe );
+    m = m_new;
+    l *= alpha;
+#pragma unroll
+    for ( int i = 0; i < 4; i++ ) {
+      p[i] = fast_exp2( p[i] - m_safe );
+      l += p[i];
+    }
+#pragma unroll
+    for ( int n = 0; n < NB; n++ ) {
+      acc[n] *= alpha;
+#pragma unroll
+      for ( int i = 0; i < 4; i++ ) {
+        acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32( to_f32( v[n][i] ), p[i], acc[n], 0, 0, 0 );
       }
     }
   }
-  if ( a.splits > 1 && lane == 0 ) {
+  l = column_sum( l );
+  for ( ; t0 < t_end; t0++ ) {
+    const T* kv = row( t0 );
+    Four<T, FOURS> k[NB], v[NB];
+    float s = 0.0f;
+#pragma unroll
+    for ( int n = 0; n < NB; n++ ) {
+      k[n].load( kv + k_off, 16 * n + 4 * g4, a.size );
+      v[n].load( kv + v_off, 16 * n + 4 * g4, a.size );
+    }
+#pragma unroll
+    for ( int n = 0; n < NB; n++ ) {
+#pragma unroll
+      for ( int e = 0; e < 4; e++ ) {
+        s = __builtin_fmaf( to_f32( x[n].e[e] ), to_f32( k[n].e[e] ), s );
+      }
+    }
+    s = column_sum( s ) * a.scale_log2e;
+    if ( t0 < my_end ) {
+      const float m_new = fmaxf( m, s ), m_safe = m_new == -INFINITY ? 0.0f : m_new, alpha = fast_exp2( m - m_safe ), w = fast_exp2( s - m_safe );
+      m = m_new;
+      l = __builtin_fmaf( l, alpha, w );
+#pragma unroll
+      for ( int n = 0; n < NB; n++ ) {
+#pragma unroll
+        for ( int i = 0; i < 4; i++ ) {
+          acc[n][i] = __builtin_fmaf( w, to_f32( v[n].e[i] ), acc[n][i] * alpha );
+        }
+      }
+    }
+  }
+  if ( !ok ) {
+    return;
+  }
+  const uint64_t slot = place * a.splits + b.split;
+#pragma unroll
+  for ( int n = 0; n < NB; n++ ) {
+#pragma unroll
+    for ( int i = 0; i < 4; i++ ) {
+      const uint32_t d = 16 * n + 4 * g4 + i;
+      if ( d < a.size ) {
+        if ( a.splits == 1 ) {
+          out[place * a.size + d] = from_f32<T>( acc[n][i] / l );
+        } else {
+          a.part_out[slot * a.size + d] = acc[n][i];
+        }
+      }
+    }
+  }
+  if ( a.splits > 1 && g4 == 0 ) {
     a.part_ml[slot * 2] = m;
     a.part_ml[slot * 2 + 1] = l;
+  }
+}
+
+// `which`: columns of a wave, which is through with storing results; masked: the first key that some column of the wave does not see, end: behind those of the work-group.
+// A function of its own so that the kernels' registers are not divided otherwise for it (inline it cost 3 to 25 %), and one for each kernel, since a function is
+// given the fewest registers of its callers': KERNEL tells them apart.
+template<typename T, int NB, bool FOURS, int KERNEL>
+__device__ __noinline__ void masked_again( const T* q, T* out, Call a, Block b, uint32_t col0, uint32_t which, uint32_t k_begin, uint32_t k_most, uint32_t masked, uint32_t end )
+{
+  if ( finite_values<T>( a.pages, b.seq, ( a.n_kv_heads + b.h ) * a.size, a.size, max( k_begin, masked ), end ) ) {
+    return;
+  }
+  __builtin_amdgcn_s_waitcnt( 0x0F70 ); // vmcnt(0): the results that are written again have been written
+  for ( ; which != 0; col0 += 16, which >>= 16 ) {
+    if ( ( which & 0xffff ) != 0 ) {
+      columns_again<T, NB, FOURS>( q, out, a, b, col0, which & 0xffff, k_begin, k_most );
+    }
   }
 }
 
@@ -144,7 +324,7 @@ struct alignas( 4 * sizeof( T ) ) Piece
 // kernel 45), a prompt of 4000 tokens 391 us (54).
 // =================================================================================================
 template<typename T, int NB, bool DECODE>
-__global__ __launch_bounds__( 256 ) void attn_pages_f32_kernel( const T* __restrict__ q, T* __restrict__ out, Call a )
+__global__ __launch_bounds__( 256, DECODE || NB == 16 ? 1 : NB == 8 ? 2 : 3 ) void attn_pages_f32_kernel( const T* __restrict__ q, T* __restrict__ out, Call a )
 {
   constexpr uint32_t HSP = 16 * NB, LD = HSP + 4, KEYS = DECODE ? 64 : 32, COLS = DECODE ? 16 : 64;
   constexpr uint32_t VR = HSP / 4;                     // pieces of a padded head
@@ -329,31 +509,7 @@ __global__ __launch_bounds__( 256 ) void attn_pages_f32_kernel( const T* __restr
   const uint64_t place = (uint64_t)( b.row0 + token ) * n_heads + head; // of the (row, head) among the outputs
   const uint64_t slot = place * a.splits + b.split;
   const bool mine = ok && k_begin < my_end;
-  if constexpr ( !DECODE ) {
-    // rows with a NaN, once more key by key
-    float probe = l;
-#pragma unroll
-    for ( int n = 0; n < NB; n++ ) {
-      probe += 0.0f * ( ( acc[n][0] + acc[n][1] ) + ( acc[n][2] + acc[n][3] ) );
-    }
-    const bool bad = mine && probe != probe;
-    uint64_t todo = __builtin_amdgcn_ballot_w64( bad );
-    todo = ( todo | todo >> 16 | todo >> 32 | todo >> 48 ) & 0xffff; // columns
-    if ( todo != 0 ) {
-      const uint32_t keep = ok && !( todo >> c & 1 );
-      for ( ; todo != 0; todo &= todo - 1 ) {
-        const uint32_t cl = b.col0 + 16 * wave + (uint32_t)__builtin_ctzll( todo );
-        walk_column<T>( q, out, a, b, cl, k_begin, min( visible( a, b, cl / a.gqa ), k_end ) );
-      }
-      if ( !keep ) {
-        return;
-      }
-    }
-  }
-  if ( !mine ) {
-    return;
-  }
-  if ( a.splits > 1 ) {
+  if ( mine && a.splits > 1 ) {
 #pragma unroll
     for ( int n = 0; n < NB; n++ ) {
 #pragma unroll
@@ -368,28 +524,41 @@ __global__ __launch_bounds__( 256 ) void attn_pages_f32_kernel( const T* __restr
       a.part_ml[slot * 2] = m;
       a.part_ml[slot * 2 + 1] = l;
     }
-    return;
-  }
-  const float inv = 1.0f / l;
+  } else if ( mine ) {
+    const float inv = 1.0f / l;
 #pragma unroll
-  for ( int n = 0; n < NB; n++ ) {
-    const uint32_t d = 16 * n + 4 * g4;
-    if ( whole ) {
-      if ( d < a.size ) {
-        Piece<T> o;
+    for ( int n = 0; n < NB; n++ ) {
+      const uint32_t d = 16 * n + 4 * g4;
+      if ( whole ) {
+        if ( d < a.size ) {
+          Piece<T> o;
+#pragma unroll
+          for ( int i = 0; i < 4; i++ ) {
+            o.e[i] = from_f32<T>( acc[n][i] * inv );
+          }
+          *reinterpret_cast<Piece<T>*>( out + place * a.size + d ) = o;
+        }
+      } else {
 #pragma unroll
         for ( int i = 0; i < 4; i++ ) {
-          o.e[i] = from_f32<T>( acc[n][i] * inv );
+          if ( d + i < a.size ) {
+            out[place * a.size + d + i] = from_f32<T>( acc[n][i] * inv );
+          }
         }
-        *reinterpret_cast<Piece<T>*>( out + place * a.size + d ) = o;
       }
-    } else {
+    }
+  }
+  if constexpr ( !DECODE ) {
+    float probe = 0.0f;
 #pragma unroll
-      for ( int i = 0; i < 4; i++ ) {
-        if ( d + i < a.size ) {
-          out[place * a.size + d + i] = from_f32<T>( acc[n][i] * inv );
-        }
-      }
+    for ( int n = 0; n < NB; n++ ) {
+      probe += 0.0f * ( ( acc[n][0] + acc[n][1] ) + ( acc[n][2] + acc[n][3] ) );
+    }
+    const uint64_t lanes = __builtin_amdgcn_ballot_w64( mine && probe != probe && l == l );
+    const uint32_t bad = (uint32_t)( lanes | lanes >> 16 | lanes >> 32 | lanes >> 48 ) & 0xffff; // columns
+    if ( bad != 0 ) {
+      const uint32_t first_col = b.col0 + 16 * wave;
+      masked_again<T, NB, false, 0>( q, out, a, b, first_col, bad, k_begin, k_begin + a.chunk, min( visible( a, b, first_col / a.gqa ), k_end ), k_end );
     }
   }
 }
@@ -432,7 +601,6 @@ constexpr float LIFT = std::is_same_v<E, __half> ? 7.0f : 0.0f;
   const unsigned r0 = r[0], r1 = r[1];
   return fmaxf( __builtin_bit_cast( float, r0 ), __builtin_bit_cast( float, r1 ) );
 }
-__device__ __forceinline__ float column_sum( float v ) { return sum_rows( sum_halves( v, v ), sum_halves( v, v ) ); }
 
 // a weight as the storage type holds it
 template<typename E>
@@ -1347,7 +1515,7 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
   }
 
   l += __shfl_xor( l, 32, WAVE );
-  float probe = l;
+  float probe = 0.0f;
 #pragma unroll
   for ( int i = 0; i < I4; i++ ) {
 #pragma unroll
@@ -1356,9 +1524,9 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
     }
   }
   const bool mine = ok && k_begin < my_end;
-  const uint64_t bad = __builtin_amdgcn_ballot_w64( mine && probe != probe );
-  uint32_t again = (uint32_t)bad | (uint32_t)( bad >> 32 ); // columns with a NaN: once more key by key
-  if ( mine && !( again >> r & 1 ) ) {
+  const uint64_t bad = __builtin_amdgcn_ballot_w64( mine && probe != probe && l == l );
+  const uint32_t again = (uint32_t)bad | (uint32_t)( bad >> 32 ); // columns
+  if ( mine ) {
     if ( a.splits > 1 ) {
       const uint64_t slot = place * a.splits + b.split;
 #pragma unroll
@@ -1390,10 +1558,8 @@ __device__ __forceinline__ void packed_run( const E* __restrict__ q, E* __restri
       }
     }
   }
-  while ( again != 0 ) {
-    const uint32_t cl = first_col + (uint32_t)__builtin_ctz( again );
-    again &= again - 1;
-    walk_column<E>( q, out, a, b, cl, k_begin, end_of( cl / a.gqa ) );
+  if ( again != 0 ) {
+    masked_again<E, CH / 2, true, 1>( q, out, a, b, first_col, again, k_begin, k_most, t_all, wg_end );
   }
 }
 
@@ -1597,14 +1763,18 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
       }
     }
   }
-  float probe = l;
+  float probe = 0.0f;
 #pragma unroll
   for ( uint32_t n = 0; n < NB; n++ ) {
     probe += 0.0f * ( ( acc[n][0] + acc[n][1] ) + ( acc[n][2] + acc[n][3] ) );
   }
   const bool mine = ok && k_begin < my_end;
-  uint64_t again = __builtin_amdgcn_ballot_w64( mine && probe != probe ); // columns with a NaN: once more key by key
-  again = ( again | again >> 16 | again >> 32 | again >> 48 ) & 0xffff;
+  const uint64_t bad = __builtin_amdgcn_ballot_w64( mine && probe != probe && l == l );
+  uint32_t again = (uint32_t)( bad | bad >> 16 | bad >> 32 | bad >> 48 ) & 0xffff; // columns
+  // (asked here as well: 4 prompts of 300 tokens, 32 heads of 128 take 45.7 us so, and 49.4 with the one call behind the stores, by how the loop's instructions fall)
+  if ( again != 0 && finite_values<float>( a.pages, b.seq, v_off / 4, a.size, max( k_begin, t_all ), wg_end ) ) {
+    again = 0;
+  }
   if ( mine && !( again >> c & 1 ) ) {
     const uint64_t slot = place * a.splits + b.split;
     const float inv = a.splits > 1 ? 1.0f : 1.0f / l;
@@ -1621,9 +1791,8 @@ __device__ __forceinline__ void packed_run_f32( const float* __restrict__ q, flo
       a.part_ml[slot * 2 + 1] = l;
     }
   }
-  for ( ; again != 0; again &= again - 1 ) {
-    const uint32_t cl = first_col + (uint32_t)__builtin_ctzll( again );
-    walk_column<float>( q, out, a, b, cl, k_begin, end_of( cl / a.gqa ) );
+  if ( again != 0 ) {
+    masked_again<float, NB, true, CG>( q, out, a, b, first_col, again, k_begin, k_most, t_all, wg_end );
   }
 }
 

@@ -1,5 +1,5 @@
-// What the kernels over a paged cache share: the address of a token's row, the sequence and tokens of a work-group's block, the walk over
-// the keys of one query row, and the checks of a description of pages.
+// What the kernels over a paged cache share: the address of a token's row, the sequence and tokens of a work-group's block, and the checks of a
+// description of pages.
 #pragma once
 
 #include "gh_common.h"
@@ -175,53 +175,6 @@ __device__ __forceinline__ uint32_t packed_sequence( const Packed& s, uint32_t r
     n += __popcll( __builtin_amdgcn_ballot_w64( i < s.batch && s.begin( i + 1 ) <= row ) );
   }
   return n < s.batch && s.begin( n ) <= row ? n : s.batch;
-}
-
-// ---- one query row by one wave, key after key -----------------------------------------------------
-// The slow form of an attention over the keys [k0, k1): scores by lanes, 64 keys at a time, then the values one by one, so that only rows that
-// are attended are touched.  The tile kernels take it for rows whose result holds a NaN: a tile multiplies the values behind a token's position by
-// a weight of zero, which makes a NaN of an infinity or a NaN there.  acc[u]: dim 64 u + lane; l is the whole sum.
-template<typename T>
-__device__ __noinline__ void walk_row( const T* q, Pages p, uint32_t seq, uint32_t kv_offset, uint32_t v_offset, uint32_t size, uint32_t k0, uint32_t k1, float scale_log2e,
-                                       float* m_out, float* l_out, float* acc )
-{
-  const uint32_t lane = threadIdx.x & 63;
-  float m = -INFINITY, l = 0.0f;
-  for ( int u = 0; u < 4; u++ ) {
-    acc[u] = 0.0f;
-  }
-  for ( uint32_t key = k0; key < k1; key += 64 ) {
-    float s = -INFINITY;
-    const T* k = reinterpret_cast<const T*>( p.row( seq, min( key + lane, k1 - 1 ) ) ) + kv_offset;
-    float dot = 0.0f;
-    for ( uint32_t d = 0; d < size; d++ ) {
-      dot = __builtin_fmaf( to_f32( q[d] ), to_f32( k[d] ), dot );
-    }
-    if ( key + lane < k1 ) {
-      s = dot * scale_log2e;
-    }
-    const float m_new = fmaxf( m, wave_max( s ) );
-    const float m_safe = m_new == -INFINITY ? 0.0f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f( m - m_safe ), w = __builtin_amdgcn_exp2f( s - m_safe );
-    m = m_new;
-    l = l * alpha + wave_sum( w );
-    for ( int u = 0; u < 4; u++ ) {
-      acc[u] *= alpha;
-    }
-    const uint32_t n = min( 64u, k1 - key );
-    for ( uint32_t j = 0; j < n; j++ ) {
-      const float wj = __shfl( w, (int)j, WAVE );
-      const T* v = reinterpret_cast<const T*>( p.row( seq, key + j ) ) + v_offset;
-      for ( int u = 0; u < 4; u++ ) {
-        const uint32_t d = 64 * u + lane;
-        if ( d < size ) {
-          acc[u] = __builtin_fmaf( wj, to_f32( v[d] ), acc[u] );
-        }
-      }
-    }
-  }
-  *m_out = m;
-  *l_out = l;
 }
 
 } // namespace gh

@@ -1,4 +1,4 @@
-"""Attention over a cache in pages at the edges of what the calls take: far positions, weights far below the largest."""
+"""Attention over a cache in pages at the edges of what the calls take: far positions, weights far below the largest, values that are no numbers."""
 import pytest
 import torch
 
@@ -7,7 +7,7 @@ from pages_plain import HALF_STEP, STEP32, Pool, attention, hold
 
 pytestmark = pytest.mark.gpu
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
-INF = float("inf")
+NAN, INF = float("nan"), float("inf")
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -21,6 +21,19 @@ def shape_of(heads, kv_heads, size):
 
 def ints(*values):
     return torch.tensor(values, dtype=torch.int32).cuda()
+
+
+def fastest(call, runs=5):
+    call()
+    times = []
+    for _ in range(runs):
+        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        begin.record()
+        call()
+        end.record()
+        torch.cuda.synchronize()
+        times.append(begin.elapsed_time(end))
+    return min(times)
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
@@ -119,3 +132,74 @@ def test_packed_scores_of_every_size(heads, kv_heads, size, dtype):
     assert bool(torch.isnan(got[60, 0]).all()) and bool(torch.isfinite(got[60, 1:]).all())
     rest = [t for t in range(tokens) if t != 60]
     hold(got[rest], want[rest], off[rest])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,size", [(8, 1, 128), (4, 4, 64), (3, 1, 256), (5, 1, 24), (4, 2, 36)])
+def test_decode_of_infinite_values(heads, kv_heads, size, dtype):
+    """An infinite value that a token attends is infinite in its result, with its sign, also in splits and beside others; two of both signs are NaN."""
+    lengths = [40, 3000, 700]
+    pool, kv = Pool(lengths, kv_heads, size, dtype), kv_heads * size
+    for i, n in enumerate(lengths):
+        rows = pool.rows[i].clone()
+        rows[n // 3, kv + 1], rows[n // 2, kv + 1], rows[n - 1, kv + 2] = INF, INF, -INF
+        rows[5, kv + 3], rows[6, kv + 3] = INF, -INF
+        pool.store(pool.table[i], rows, 0)
+    q = torch.randn((len(lengths), heads * size), generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
+    xb = torch.zeros_like(q)
+    ops.attn_decode_paged(q, ops.pages(pool.pool, pool.table), ints(*lengths), xb, max(lengths), shape_of(heads, kv_heads, size))
+    got = xb.reshape(len(lengths), heads, size)
+    group = got[:, :heads // kv_heads]
+    assert bool((group[:, :, 1] == INF).all()) and bool((group[:, :, 2] == -INF).all()) and bool(torch.isnan(group[:, :, 3]).all())
+    assert bool(torch.isfinite(group[:, :, 4:]).all()) and bool(torch.isfinite(got[:, heads // kv_heads:]).all())
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,size,tokens", [(F16, 8, 1, 128, 2048), (BF16, 8, 8, 64, 2048), (F16, 4, 1, 256, 1024), (F32, 8, 8, 64, 1024), (F32, 4, 2, 128, 1024),
+                                                              (F16, 8, 4, 36, 1024)])
+@pytest.mark.parametrize("what", ["row", "values", "every value", "one dim"])
+def test_a_poisoned_prompt_is_no_long_call(what, dtype, heads, kv_heads, size, tokens):
+    """NaN near a prompt's beginning reaches every token from there on and none before, in a call about as long as another, and the next sequence is as it was."""
+    kv, other, bad = kv_heads * size, 50, 37
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pages = -(-tokens // 16)
+    pool = torch.randn((pages + 4, 16, 2 * kv), generator=g, device="cuda").to(dtype)
+    table = torch.zeros((2, pages), dtype=torch.int32, device="cuda")
+    table[0] = torch.arange(pages)
+    table[1, :4] = torch.arange(pages, pages + 4)
+    q = torch.randn((tokens + other, heads * size), generator=g, device="cuda").to(dtype)
+    first, shape = ints(0, tokens, tokens + other), shape_of(heads, kv_heads, size)
+    room = torch.empty(max(16, ops.attn_packed_workspace(2, tokens + other, tokens, shape, dtype)), dtype=torch.uint8, device="cuda")
+
+    def run(xb):
+        ops.attn_packed(q, ops.pages(pool, table), first, None, xb, tokens, shape, room)
+        return xb
+
+    clean = run(torch.full_like(q, 7.0))
+    usual = fastest(lambda: run(torch.empty_like(q)))
+    rows = pool[:pages].reshape(-1, 2 * kv)
+    if what == "row":
+        rows[bad] = NAN
+    elif what == "values":
+        rows[bad, kv:] = NAN
+    elif what == "every value":
+        rows[bad:, kv:] = INF
+    else:
+        rows[bad, kv + 1] = NAN
+    got = run(torch.full_like(q, 7.0))
+    poisoned = fastest(lambda: run(torch.empty_like(q)))
+    a, b = got.reshape(-1, heads, size), clean.reshape(-1, heads, size)
+    assert torch.equal(a[tokens:], b[tokens:]), "the other sequence"
+    # rows of the same keys in another way of summing: both within what rounding allows of the exact result
+    want, off = attention(q[:bad].reshape(bad, heads, size), rows[:bad, :kv].double().reshape(bad, kv_heads, size), rows[:bad, kv:].double().reshape(bad, kv_heads, size), 0, dtype, dtype != F32)
+    hold(a[:bad], want, off, "before the bad token")
+    later, group = a[bad:tokens], heads // kv_heads
+    if what in ("row", "values"):
+        assert bool(torch.isnan(later).all())
+    elif what == "every value":
+        assert bool(torch.isinf(later).all())
+    else:
+        assert bool(torch.isnan(later[:, :group, 1]).all())
+        keep = torch.ones((heads, size), dtype=torch.bool, device="cuda")
+        keep[:group, 1] = False
+        assert float((later[:, keep].double() - b[bad:tokens][:, keep].double()).abs().max()) <= 8 * HALF_STEP[dtype] * 4 + 4000 * STEP32
+    assert poisoned < 25 * usual, f"{poisoned * 1e3:.0f} us, without NaN {usual * 1e3:.0f}"
