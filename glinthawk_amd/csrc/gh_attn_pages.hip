@@ -1914,7 +1914,7 @@ Plan plan_call( bool decode, uint64_t batch, uint64_t rows, uint32_t max_keys, c
 {
   Plan p {};
   uint32_t cols = decode ? 16 : tiles && dt != GH_F32 ? 128 : 64;
-  auto blocks_of = [&] { return std::min<uint64_t>( ( rows * s->gqa_size + cols - 1 ) / cols + batch, rows * s->gqa_size ); };
+  auto blocks_of = [&] { return most_blocks( rows * s->gqa_size, batch, cols ); };
   // fp32: half as many columns a work-group while there are fewer than two and a half a CU, since a launch of few lasts as long as its longest (5 prompts of 100 to 900 tokens, 12
   // heads of 64: 51 us with 64 columns, 40 with 32; 4 of 300, 32 heads of 128: 46 and 49; 16 of 1000, 12 heads of 64: 254 and 294)
   if ( !decode && tiles && dt == GH_F32 && blocks_of() * s->n_kv_heads * 2 < 5ull * (uint64_t)cu_count() ) {

@@ -14,15 +14,7 @@ __global__ __launch_bounds__( 256 ) void page_rows_kernel( Pages p, Packed s, vo
   if ( t >= s.tokens ) {
     return;
   }
-  uint32_t low = 0, high = s.batch; // begin( low ) <= t < begin( high ), or no sequence has the token
-  while ( high - low > 1 ) {
-    const uint32_t middle = ( low + high ) / 2;
-    if ( s.begin( middle ) <= t ) {
-      low = middle;
-    } else {
-      high = middle;
-    }
-  }
+  const uint32_t low = last_at_most( s.batch, t, [&]( uint32_t i ) { return s.begin( i ); } );
   const bool has = s.begin( low ) <= t && t < s.begin( low + 1 );
   const uint64_t pos = ( has && s.start ? (uint64_t)s.start[low] : 0 ) + ( has ? t - s.begin( low ) : 0 );
   void* row = nullptr;

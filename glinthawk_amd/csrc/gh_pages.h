@@ -88,20 +88,56 @@ __device__ __forceinline__ uint32_t wave_max_u32( uint32_t v )
   return wave_all( v, []( uint32_t a, uint32_t b ) { return a > b ? a : b; } );
 }
 
-// Block number -> (sequence, block of the sequence), by a whole wave.  A sequence of n tokens with `gqa` columns each has ceil(n gqa / columns) blocks.  Blocks are
-// numbered by falling level, which is the block's place in its sequence plus the blocks that the sequence's start position would be, so that the ones with the most
-// keys come first and a launch does not end on a long one.  The level of a number is found by bisection over how many blocks lie at a level and above, a sum over the
-// sequences.  False: no such block.
+// The last sequence i with key( i ) <= value, for keys that do not fall; 0 if there is none.
+template<typename Key>
+__device__ __forceinline__ uint32_t last_at_most( uint32_t batch, uint32_t value, Key key )
+{
+  uint32_t low = 0, high = batch;
+  while ( high - low > 1 ) {
+    const uint32_t middle = ( low + high ) / 2;
+    if ( key( middle ) <= value ) {
+      low = middle;
+    } else {
+      high = middle;
+    }
+  }
+  return low;
+}
+
 // A sequence as packed_block found it
 struct PackedBlock
 {
   uint32_t seq, block;
   uint32_t row0, tokens, start; // of the sequence
 };
+
+// Block number -> (sequence, block of the sequence), by a whole wave.  A sequence of n tokens with `gqa` columns each has ceil(n gqa / columns) blocks.  Blocks are
+// numbered by falling level, which is the block's place in its sequence plus the blocks that the sequence's start position would be, so that the ones with the most
+// keys come first and a launch does not end on a long one.  The level of a number is found by bisection over how many blocks lie at a level and above, a sum over the
+// sequences.  False: no such block.
+// Every block reads all sequences for that, so where there are many numbers go by the sequences' places: sequence i has those from floor(first[i] gqa / columns) + i on,
+// at least as many as it has blocks, and its last block comes first.  In order and by place, us: f16, 64 heads on 8 of 128, 1 to 300 tokens each: 65 sequences 175 and
+// 148, 200 564 and 385, 500 1858 and 927; 200 of one token behind 1000 keys 143 and 123, 2000 2590 and 1017; 64 and fewer are kept in registers.
+// fp32, 12 heads of 64, where a block takes longer and fewer run at a time: one token behind 0 to 2000 keys, 100 sequences 148 and 170, 200 281 and 295, 500 908 and 665;
+// 1 to 300 tokens, 200 sequences 281 and 207.
+__host__ __device__ constexpr uint32_t most_ordered( uint32_t columns ) { return columns == 128 ? 64 : 256; } // 128: of the 16-bit kernel
+// numbers of blocks there may be: a block has a column, and all but the last of a sequence are full
+__host__ __device__ constexpr uint64_t most_blocks( uint64_t all_columns, uint64_t batch, uint32_t columns )
+{
+  return ( all_columns + columns - 1 ) / columns + batch < all_columns ? ( all_columns + columns - 1 ) / columns + batch : all_columns;
+}
 __device__ __forceinline__ bool packed_block( const Packed& s, uint32_t gqa, uint32_t columns, uint32_t number, PackedBlock* found )
 {
   const uint32_t lane = threadIdx.x & 63;
   auto blocks_of = [&]( uint32_t tokens ) { return (uint32_t)( ( (uint64_t)tokens * gqa + columns - 1 ) / columns ); };
+  if ( s.batch > most_ordered( columns ) ) {
+    // where there are fewer columns than such numbers, a number is a column's, and the block's that it begins
+    const bool by_column = most_blocks( (uint64_t)s.tokens * gqa, s.batch, columns ) == (uint64_t)s.tokens * gqa;
+    auto slot = [&]( uint32_t i ) { return by_column ? s.begin( i ) * gqa : (uint32_t)( (uint64_t)s.begin( i ) * gqa / columns ) + i; };
+    const uint32_t i = last_at_most( s.batch, number, slot ), n = blocks_of( s.count( i ) ), place = number - slot( i );
+    *found = { i, by_column ? place / columns : n - 1 - place, s.begin( i ), s.count( i ), s.begin_pos( i ) };
+    return slot( i ) <= number && ( by_column ? place < s.count( i ) * gqa && place % columns == 0 : place < n );
+  }
   auto blocks = [&]( uint32_t i ) { return i < s.batch ? blocks_of( s.count( i ) ) : 0u; };
   auto level_of = [&]( uint32_t start ) { return (uint32_t)min( (uint64_t)start * gqa / columns, (uint64_t)0x3fffffff ); }; // of a sequence's first block
   auto level0 = [&]( uint32_t i ) { return i < s.batch ? level_of( s.begin_pos( i ) ) : 0u; };
@@ -166,15 +202,17 @@ __device__ __forceinline__ bool packed_block( const Packed& s, uint32_t gqa, uin
   return false;
 }
 
-// The sequence a packed row belongs to, by a whole wave: as many sequences as end at or before it lie in front.  batch: none.
+// The sequence a packed row belongs to, by a whole wave; batch: none.
 __device__ __forceinline__ uint32_t packed_sequence( const Packed& s, uint32_t row )
 {
-  uint32_t n = 0;
-  for ( uint32_t i0 = 0; i0 < s.batch; i0 += 64 ) {
-    const uint32_t i = i0 + ( threadIdx.x & 63 );
-    n += __popcll( __builtin_amdgcn_ballot_w64( i < s.batch && s.begin( i + 1 ) <= row ) );
+  uint32_t i;
+  if ( s.batch <= 64 ) { // as many sequences as end at or before it lie in front
+    const uint32_t lane = threadIdx.x & 63;
+    i = __popcll( __builtin_amdgcn_ballot_w64( lane < s.batch && s.begin( lane + 1 ) <= row ) );
+  } else {
+    i = last_at_most( s.batch, row, [&]( uint32_t k ) { return s.begin( k ); } );
   }
-  return n < s.batch && s.begin( n ) <= row ? n : s.batch;
+  return i < s.batch && s.begin( i ) <= row && row < s.begin( i + 1 ) ? i : s.batch;
 }
 
 } // namespace gh

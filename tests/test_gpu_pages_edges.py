@@ -1,4 +1,4 @@
-"""Attention over a cache in pages at the edges of what the calls take: far positions, weights far below the largest, values that are no numbers."""
+"""Attention over a cache in pages at the edges of what the calls take: far positions, weights far below the largest, values that are no numbers, many sequences."""
 import pytest
 import torch
 
@@ -203,3 +203,40 @@ def test_a_poisoned_prompt_is_no_long_call(what, dtype, heads, kv_heads, size, t
         keep[:group, 1] = False
         assert float((later[:, keep].double() - b[bad:tokens][:, keep].double()).abs().max()) <= 8 * HALF_STEP[dtype] * 4 + 4000 * STEP32
     assert poisoned < 25 * usual, f"{poisoned * 1e3:.0f} us, without NaN {usual * 1e3:.0f}"
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,size", [(F16, 8, 1, 128), (BF16, 4, 4, 64), (F32, 4, 2, 64), (F16, 4, 2, 36)])
+@pytest.mark.parametrize("batch", [64, 65, 256, 257, 3000])
+@pytest.mark.parametrize("tokens", [(0, 1, 1, 5, 0, 33, 1), (1, 0, 1, 1), (0,) * 10 + (2,)])
+def test_many_sequences(tokens, batch, dtype, heads, kv_heads, size):
+    """Single tokens, prompts and sequences without tokens in one call, contexts that share pages; and nothing of the rows behind."""
+    new = [tokens[i % len(tokens)] for i in range(batch)]
+    past = [(i * 37) % 90 for i in range(batch)]
+    pool = Pool([130], kv_heads, size, dtype)
+    table = pool.table.expand(batch, -1).contiguous()
+    first = torch.tensor([0] + new).cumsum(0).int().cuda()
+    q = torch.randn((sum(new) + 3, heads * size), generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    xb = torch.full_like(q, 7.0)
+    ops.attn_packed(q, ops.pages(pool.pool, table), first, ints(*past), xb, 130, shape_of(heads, kv_heads, size))
+    assert bool((xb[sum(new):] == 7.0).all()) and bool((xb[:sum(new)] != 7.0).any(1).all())
+    group = heads // kv_heads
+    k, v = pool.k(0).repeat_interleave(group, 1), pool.v(0).repeat_interleave(group, 1)
+    where = torch.tensor([past[i] + t for i in range(batch) for t in range(new[i])], device="cuda")
+    x = q[:sum(new)].double().reshape(-1, heads, size)
+    scores = (x.transpose(0, 1).float().double() @ k.permute(1, 2, 0).contiguous()) * size ** -0.5                     # (heads, tokens, keys)
+    w = torch.softmax(scores.masked_fill(torch.arange(130, device="cuda") > where[:, None], -INF), -1)
+    v = v.transpose(0, 1).contiguous()
+    want, mean = (w @ v).transpose(0, 1), (w @ v.abs()).transpose(0, 1)
+    off = mean * (3 * HALF_STEP[dtype] + 2 * (size + 16 + 130) * STEP32 * (1 + float(scores.abs().max()))) + HALF_STEP[dtype] * want.abs() + (200 * 2.0 ** -25 * 4 if dtype == F16 else 0)
+    hold(xb[:sum(new)].reshape(-1, heads, size), want, off)
+
+
+def test_the_time_of_many_sequences_grows_with_their_number():
+    times = {}
+    for batch in (512, 4096):
+        pool = torch.randn((64, 16, 2048), device="cuda").half()
+        table = torch.randint(64, (batch, 4), dtype=torch.int32, device="cuda")
+        q, first, start = torch.randn((batch, 8192), device="cuda").half(), torch.arange(batch + 1, dtype=torch.int32, device="cuda"), torch.full((batch,), 40, dtype=torch.int32, device="cuda")
+        xb, p, shape = torch.empty_like(q), ops.pages(pool, table), shape_of(64, 8, 128)
+        times[batch] = fastest(lambda: ops.attn_packed(q, p, first, start, xb, 64, shape))
+    assert times[4096] < 2 * 8 * times[512], times
