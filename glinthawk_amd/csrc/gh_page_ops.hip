@@ -2,6 +2,7 @@
 #include "gh_pages.h"
 
 #include <algorithm>
+#include <new>
 #include <vector>
 
 namespace gh {
@@ -142,7 +143,12 @@ int gh_copy_pages_host( void* pool, uint64_t page_stride, uint64_t page_bytes, u
     if ( int rc = check_copy( "gh_copy_pages_host", pool, page_stride, page_bytes, n_pages, layers, layer_stride, pairs_host, n_pairs ) ) {
       return rc;
     }
-    std::vector<uint32_t> written( n_pairs );
+    std::vector<uint32_t> written;
+    try {
+      written.resize( n_pairs );
+    } catch ( const std::bad_alloc& ) {
+      return fail( GH_ERR_OOM, "gh_copy_pages_host: no memory to check %llu pairs", (unsigned long long)n_pairs );
+    }
     for ( uint64_t j = 0; j < n_pairs; j++ ) {
       GH_REQUIRE( pairs_host[2 * j] < n_pages && pairs_host[2 * j + 1] < n_pages, "gh_copy_pages_host: pair %llu, %u to %u, of %u pages", (unsigned long long)j,
                   pairs_host[2 * j], pairs_host[2 * j + 1], n_pages );
