@@ -448,6 +448,13 @@ def _stream_on(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _u32(**numbers: int) -> None:
+    """Refuses what ctypes would cut to 32 bits."""
+    for name, n in numbers.items():
+        if not 0 <= n < 2 ** 32:
+            raise ValueError(f"{name}: {n} does not fit 32 bits")
+
+
 @functools.lru_cache(maxsize=None)
 def _shape_ref(shape: Shape):
     return C.byref(shape.c())
@@ -480,12 +487,15 @@ def page_rows(p: GhPages, first: torch.Tensor, start_pos: Optional[torch.Tensor]
 
 def attn_decode_paged_workspace(batch: int, max_length: int, shape: Shape, dtype: torch.dtype) -> int:
     """Bytes that serve every call of at most so many contexts and keys."""
+    _u32(max_length=max_length)
     return int(lib().gh_attn_decode_paged_workspace(batch, max_length, _shape_ref(shape), _dt(torch.empty(0, dtype=dtype))))
 
 
 def attn_decode_paged(q: torch.Tensor, p: GhPages, lengths: torch.Tensor, xb: torch.Tensor, max_length: int, shape: Shape,
                       workspace: Optional[torch.Tensor] = None) -> None:
     batch = q.shape[0]
+    if not 0 <= max_length < 2 ** 32:
+        _u32(max_length=max_length)
     if not (q.dtype is p.dtype and xb.dtype is p.dtype and lengths.dtype is torch.int32 and q.shape == (batch, shape.dim) and xb.shape == q.shape and lengths.shape == (batch,)
             and q.is_contiguous() and xb.is_contiguous() and lengths.is_contiguous() and q.device == p.device and xb.device == p.device and lengths.device == p.device
             and (workspace is None or (workspace.device == p.device and workspace.is_contiguous())) and p.contexts >= batch and p.row == 2 * shape.kv_dim):
@@ -499,6 +509,7 @@ def attn_decode_paged(q: torch.Tensor, p: GhPages, lengths: torch.Tensor, xb: to
 
 def attn_packed_workspace(batch: int, n_tokens: int, max_keys: int, shape: Shape, dtype: torch.dtype) -> int:
     """Bytes that serve every call of at most so many sequences, tokens and keys."""
+    _u32(max_keys=max_keys)
     return int(lib().gh_attn_packed_workspace(batch, n_tokens, max_keys, _shape_ref(shape), _dt(torch.empty(0, dtype=dtype))))
 
 
@@ -506,6 +517,8 @@ def attn_packed(q: torch.Tensor, p: GhPages, first: torch.Tensor, start_pos: Opt
                 workspace: Optional[torch.Tensor] = None) -> None:
     """first: (sequences + 1) int32, where each sequence's tokens begin in q and xb; start_pos: (sequences) int32 or None."""
     tokens, batch = q.shape[0], first.numel() - 1
+    if not 0 <= max_keys < 2 ** 32:
+        _u32(max_keys=max_keys)
     if not (q.dtype is p.dtype and xb.dtype is p.dtype and first.dtype is torch.int32 and q.shape == (tokens, shape.dim) and xb.shape == q.shape and first.shape == (batch + 1,)
             and q.is_contiguous() and xb.is_contiguous() and first.is_contiguous() and q.device == p.device and xb.device == p.device and first.device == p.device
             and (start_pos is None or (start_pos.dtype is torch.int32 and start_pos.shape == (batch,) and start_pos.is_contiguous() and start_pos.device == p.device))
@@ -538,6 +551,7 @@ def copy_pages(pool: torch.Tensor, pairs) -> None:
 
 
 def token_logprobs_workspace(rows: int, vocab: int, n_top: int) -> int:
+    _u32(n_top=n_top)
     return int(lib().gh_token_logprobs_workspace(rows, vocab, n_top))
 
 
@@ -547,6 +561,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, n_top: int = 0, w
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise ValueError("rows of logits lie with their values one behind the other")
     (rows, vocab), device = logits.shape, logits.device
+    if not 0 <= n_top <= vocab:
+        raise ValueError(f"{n_top} alternatives of {vocab} values")
     if not (tokens.dtype is torch.int32 and tokens.shape == (rows,) and tokens.is_contiguous() and tokens.device == device
             and (workspace is None or (workspace.device == device and workspace.is_contiguous()))):
         _refuse(logits, tokens=(tokens, torch.int32, (rows,)), workspace=(workspace, None if workspace is None else workspace.dtype, () if workspace is None else workspace.shape))

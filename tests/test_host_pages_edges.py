@@ -2,7 +2,11 @@
 import subprocess
 import sys
 
+import pytest
+import torch
+
 import glinthawk_amd
+from glinthawk_amd import Shape, ops
 
 FAILING = r"""
 import ctypes, resource, sys
@@ -23,3 +27,18 @@ def test_pairs_that_memory_does_not_suffice_for_are_refused():
     assert ran.returncode == 0, (ran.returncode, ran.stderr)
     rc, said = ran.stdout.split(" ", 1)
     assert int(rc) < 0 and "no memory" in said
+
+
+@pytest.mark.parametrize("most", [2 ** 32, 2 ** 32 + 16, -1, 2 ** 40])
+def test_bounds_that_32_bits_do_not_hold_are_refused(most):
+    """They are not cut to a smaller bound, whose keys alone would be attended."""
+    shape = Shape(dim=1024, n_layers=1, n_heads=8, n_kv_heads=2, hidden_dim=8, seq_len=8)
+    p = ops.pages(torch.zeros(4, 16, 512, dtype=torch.float16), torch.zeros((2, 3), dtype=torch.int32))
+    q, ints, room = torch.zeros(2, 1024, dtype=torch.float16), torch.ones(3, dtype=torch.int32), torch.zeros(16, dtype=torch.uint8)
+    for call in (lambda: ops.attn_decode_paged(q, p, ints[:2], q.clone(), most, shape, room), lambda: ops.attn_packed(q, p, ints, None, q.clone(), most, shape, room),
+                 lambda: ops.attn_decode_paged_workspace(2, most, shape, torch.float16), lambda: ops.attn_packed_workspace(2, 9, most, shape, torch.float16),
+                 lambda: ops.token_logprobs_workspace(2, 100, most)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+    with pytest.raises(ValueError, match="alternatives"):
+        ops.token_logprobs(torch.zeros(2, 9), ints[:2], most, room)
