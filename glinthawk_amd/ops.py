@@ -455,7 +455,7 @@ def _u32(**numbers: int) -> None:
             raise ValueError(f"{name}: {n} does not fit 32 bits")
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache(maxsize=64)      # of the shapes a program goes on with
 def _shape_ref(shape: Shape):
     return C.byref(shape.c())
 

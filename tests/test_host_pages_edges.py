@@ -42,3 +42,10 @@ def test_bounds_that_32_bits_do_not_hold_are_refused(most):
             call()
     with pytest.raises(ValueError, match="alternatives"):
         ops.token_logprobs(torch.zeros(2, 9), ints[:2], most, room)
+
+
+def test_descriptors_of_many_shapes_are_not_all_kept():
+    for n in range(1, 300):
+        shape = Shape(dim=8 * n, n_layers=1, n_heads=n, n_kv_heads=n, hidden_dim=8, seq_len=8)
+        assert ops.attn_decode_paged_workspace(1, 128, shape, torch.float16) == 2 * n * (8 + 2) * 4
+    assert ops._shape_ref.cache_info().currsize <= 64
