@@ -49,3 +49,19 @@ def test_descriptors_of_many_shapes_are_not_all_kept():
         shape = Shape(dim=8 * n, n_layers=1, n_heads=n, n_kv_heads=n, hidden_dim=8, seq_len=8)
         assert ops.attn_decode_paged_workspace(1, 128, shape, torch.float16) == 2 * n * (8 + 2) * 4
     assert ops._shape_ref.cache_info().currsize <= 64
+
+
+@pytest.mark.parametrize("heads,kv_heads,size", [(8, 2, 128), (64, 8, 128), (6, 6, 48), (33, 1, 64), (2, 2, 256)])
+def test_workspaces_of_larger_calls_cover_smaller_ones(heads, kv_heads, size):
+    """No smaller batch, number of tokens or bound asks for more, across the 64 keys that take no splits and the bound of partial results."""
+    shape = Shape(dim=heads * size, n_layers=1, n_heads=heads, n_kv_heads=kv_heads, hidden_dim=8, seq_len=8)
+    rows, keys = [1, 2, 3, 15, 16, 17, 63, 64, 100, 255, 1000, 1023, 1024, 4000, 70000], [0, 1, 63, 64, 65, 128, 129, 1000, 4096, 40000, 2 ** 24, 2 ** 31 - 1]
+    for size_of in (lambda n, k: ops.attn_decode_paged_workspace(n, k, shape, torch.float16), lambda n, k: ops.attn_packed_workspace(min(n, 3), n, k, shape, torch.float16)):
+        table = [[size_of(n, k) for k in keys] for n in rows]
+        assert all(a <= b for line in table for a, b in zip(line, line[1:])) and all(a <= b for low, high in zip(table, table[1:]) for a, b in zip(low, high))
+        assert all(v == 0 for line in table for v in line[:4]) and 0 < table[0][4] and table[-1][-1] <= 65536 * (size + 2) * 4
+    for vocab in (1, 100, 32768, 32769, 65537, 130001, 2 ** 21):
+        tops = [n for n in (0, 1, 5, 20, 64) if n <= vocab]
+        table = [[ops.token_logprobs_workspace(n, vocab, k) for k in tops] for n in (1, 2, 7, 300, 65535)]
+        assert all(a <= b for line in table for a, b in zip(line, line[1:])) and all(a <= b for low, high in zip(table, table[1:]) for a, b in zip(low, high))
+        assert all((v == 0) == (vocab <= 32768) for line in table for v in line)
