@@ -64,3 +64,15 @@ def test_log_probabilities_are_never_above_zero(dtype):
     x[:, 5] = torch.linspace(15, 60, 4000).to(dtype).cuda()
     given, entropy, _, top = ops.token_logprobs(x, torch.full((4000,), 5, dtype=torch.int32, device="cuda"), 2)
     assert bool((given <= 0).all()) and bool((top <= 0).all()) and bool((entropy >= 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_alternatives_of_a_product(dtype):
+    """Logits as the dense product gives them: the alternatives' indices in every type, the first of them what the argmax says where that takes the type."""
+    g = torch.Generator().manual_seed(4)
+    x, w = torch.randn((4, 512), generator=g).to(dtype).cuda(), torch.randn((777, 512), generator=g).to(dtype).cuda()
+    logits = ops.matmul(x, w)
+    ids = ops.token_logprobs(logits, torch.tensor([0, 5, 776, 100], dtype=torch.int32).cuda(), 7)[2]
+    assert torch.equal(ids.long(), logprobs(logits, torch.zeros(4, dtype=torch.int32).cuda(), 7)[2])
+    if dtype != BF16:
+        assert ops.argmax(logits) == ids[:, 0].tolist()
