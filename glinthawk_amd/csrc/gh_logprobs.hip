@@ -10,8 +10,10 @@
 // work-groups of a CU are in different phases already.
 // The largest values: of the threads' own largest, each wave finds one that q of its threads reach and few more; half the waves have q threads that reach the middle one of
 // those, so with q = 2 n / waves at least n values do, and of many thousand only some more.  They go to LDS as whole numbers, a value's bits in the order of the values, then its index the other way
-// round, so that no two are equal and the lower index of equal values is the larger number, and are ranked by counting; where they are more than fit, the numbers come
-// out one after the other, each the largest below the one before.
+// round, so that no two are equal and the lower index of equal values is the larger number, and are ranked by counting.  Where they are more than fit since many are equal
+// (a row that lets few tokens through is -inf elsewhere), the row is read again for what is larger and for as many of the equal ones as are wanted: 2047 rows of which
+// 30 of 32000 f16 values are finite, 20 alternatives, 102 us a call on its own (50 with all of them finite).  Where even what is larger is more than fit (a row whose
+// values are in order), the numbers come out one after the other, each the largest below the one before.
 // Rows of one part are finished by their work-group.  Longer ones are cut into parts whose S, T, m and sorted largest numbers a second kernel joins.
 #include "gh_common.h"
 
@@ -158,7 +160,7 @@ __global__ __launch_bounds__( THREADS, THREADS == 512 || ( THREADS == 1024 && PI
   __shared__ float2 s_sums[WAVES];
   __shared__ float s_best[WAVES], s_reach[WAVES];
   __shared__ uint64_t s_number[CANDIDATES];
-  __shared__ uint32_t s_count;
+  __shared__ uint32_t s_count, s_found[WAVES];
   const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
   const uint64_t row = blockIdx.y;
   const T* x = logits + row * row_stride;
@@ -224,6 +226,7 @@ __global__ __launch_bounds__( THREADS, THREADS == 512 || ( THREADS == 1024 && PI
   if ( lane == 0 ) {
     s_sums[wave] = make_float2( wave_s, wave_t );
   }
+  float reach = 0.0f;
   if ( n_top != 0 ) {
     // the middle one of the waves' values: as many are larger, or equal and in front
     const float mine = s_reach[lane % WAVES];
@@ -233,7 +236,7 @@ __global__ __launch_bounds__( THREADS, THREADS == 512 || ( THREADS == 1024 && PI
       const float other = lane_value( mine, (int)w );
       rank += other > mine || ( other == mine && w < lane );
     }
-    const float reach = lane_value( mine, __builtin_ctzll( __builtin_amdgcn_ballot_w64( rank == WAVES / 2 - 1 ) ) );
+    reach = lane_value( mine, __builtin_ctzll( __builtin_amdgcn_ballot_w64( rank == WAVES / 2 - 1 ) ) );
     uint32_t thread = threadIdx.x;
     asm volatile( "" : "+v"( thread ) ); // (the columns' numbers are made here and not ahead of time)
     if ( !( best < reach ) ) { // few threads come this far
@@ -287,19 +290,61 @@ __global__ __launch_bounds__( THREADS, THREADS == 512 || ( THREADS == 1024 && PI
       o.top_logprobs[row * n_top + rank] = ( value_of( number ) - m ) - log_s;
     }
   };
-  if ( count <= CANDIDATES ) {
-    for ( uint32_t i = threadIdx.x; i < count; i += THREADS ) {
+  uint32_t listed = count;
+  if ( count > CANDIDATES ) {
+    // More than fit, since many are equal to what is reached (a row that lets few tokens through is -inf elsewhere): the row once more, for what is larger, and then, in the order
+    // of their columns and no further than they are wanted, for what is equal; behind -inf for NaN.
+    __syncthreads();
+    if ( threadIdx.x == 0 ) {
+      s_count = 0;
+    }
+    __syncthreads();
+    for ( uint32_t i = threadIdx.x; i < n; i += THREADS ) {
+      const float v = to_f32( x[c0 + i] );
+      if ( v > reach ) {
+        const uint32_t at = atomicAdd( &s_count, 1u );
+        if ( at < CANDIDATES ) {
+          s_number[at] = number_of( v, i );
+        }
+      }
+    }
+    __syncthreads();
+    listed = s_count;
+    for ( uint32_t look = 0; look < ( reach == -INFINITY ? 2u : 1u ) && listed < n_top; look++ ) {
+      for ( uint32_t i0 = 0; i0 < n && listed < n_top; i0 += THREADS ) {
+        const uint32_t i = i0 + threadIdx.x;
+        const float v = i < n ? to_f32( x[c0 + i] ) : 0.0f;
+        const uint64_t have = __builtin_amdgcn_ballot_w64( i < n && ( look == 0 ? v == reach : v != v ) );
+        if ( lane == 0 ) {
+          s_found[wave] = __popcll( have );
+        }
+        __syncthreads();
+        uint32_t at = listed + __popcll( have & ( ( 1ull << lane ) - 1 ) );
+        for ( uint32_t w = 0; w < WAVES; w++ ) {
+          at += w < wave ? s_found[w] : 0;
+          listed += s_found[w];
+        }
+        if ( ( have >> lane & 1 ) && at < n_top ) {
+          s_number[at] = number_of( v, i );
+        }
+        __syncthreads();
+      }
+    }
+    listed = s_count >= n_top ? s_count : min( listed, n_top ); // (of the equal ones no more than are wanted were put down)
+  }
+  if ( listed <= CANDIDATES ) {
+    for ( uint32_t i = threadIdx.x; i < listed; i += THREADS ) {
       const uint64_t number = s_number[i];
       uint32_t rank = 0;
 #pragma unroll 8
-      for ( uint32_t k = 0; k < count; k++ ) {
+      for ( uint32_t k = 0; k < listed; k++ ) {
         rank += s_number[k] > number;
       }
       if ( rank < n_top ) {
         put( rank, number );
       }
     }
-    for ( uint32_t i = count + threadIdx.x; i < n_top; i += THREADS ) { // a part of fewer columns than alternatives
+    for ( uint32_t i = listed + threadIdx.x; i < n_top; i += THREADS ) { // a part of fewer columns than alternatives
       put( i, 0 );
     }
     return;

@@ -76,3 +76,54 @@ def test_alternatives_of_a_product(dtype):
     assert torch.equal(ids.long(), logprobs(logits, torch.zeros(4, dtype=torch.int32).cuda(), 7)[2])
     if dtype != BF16:
         assert ops.argmax(logits) == ids[:, 0].tolist()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("vocab", [1500, 5000, 32000, 70001])
+def test_rows_that_let_few_tokens_through(vocab, dtype):
+    """Grammar masks: some values, -inf elsewhere, NaN among it or not, fewer values than alternatives or more, in one place or apart; and rows where most values are equal."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn((12, vocab), generator=g)
+    rows = torch.full((12, vocab), -INF)
+    for row, allowed in enumerate((range(100, 130), [vocab - 1], range(3, vocab, vocab // 5), range(0, vocab, 3), [], range(vocab - 70, vocab), [0, 1, 2])):
+        rows[row, list(allowed)] = x[row, list(allowed)]
+    rows[7] = 2.0
+    rows[7, 40:vocab:700] = 3.0
+    rows[8] = torch.where(x[8] > 1.5, x[8], 1.0)
+    rows[9] = -0.0
+    rows[9, ::2] = 0.0
+    rows[9, 77] = -1.0
+    rows[10, 5:9] = x[10, 5:9]
+    rows[10, vocab // 2:] = float("nan")
+    rows[11] = float("nan")
+    rows[11, vocab - 2] = 1.0
+    rows[11, 300] = -INF
+    rows = rows.to(dtype).cuda()
+    for n_top in (1, 5, 20, 64):
+        ids = ops.token_logprobs(rows, torch.zeros(12, dtype=torch.int32, device="cuda"), n_top)[2]
+        want = logprobs(rows, torch.zeros(12, dtype=torch.int32, device="cuda"), n_top)[2]
+        for row in range(12):
+            assert ids[row].tolist() == want[row].tolist(), (row, n_top)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("n_top", [5, 64])
+def test_rows_that_let_few_tokens_through_are_no_long_call(n_top, dtype):
+    x = torch.randn((1000, 32000), device="cuda").to(dtype)
+    masked = torch.full_like(x, -INF)
+    masked[:, 100:130] = x[:, 100:130]
+    tokens = torch.zeros(1000, dtype=torch.int32, device="cuda")
+
+    def fastest(logits):
+        times = []
+        for _ in range(5):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            ops.token_logprobs(logits, tokens, n_top)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        return min(times[1:])
+
+    usual, few = fastest(x), fastest(masked)
+    assert few < 6 * usual, f"{few * 1e3:.0f} us, without a mask {usual * 1e3:.0f}"
