@@ -321,7 +321,7 @@ struct alignas( 4 * sizeof( T ) ) Piece
 // The next stage's rows are asked for before a stage is computed.
 // Taken where rows cannot go straight to LDS in pieces of 16 bytes: head sizes that are no multiple of them, pages below 16 tokens, pool or rows that are not aligned.
 // Bound by its own conversions and LDS traffic.  f16, 8 heads on 4 kv heads of 36: decode of 64 contexts of 100 to 4000 keys 94 us (0.8 TB/s; heads of 40 in the streaming
-// kernel 45), a prompt of 4000 tokens 391 us (54).
+// kernel 45), a prompt of 4000 tokens 376 us (53).
 // =================================================================================================
 template<typename T, int NB, bool DECODE>
 __global__ __launch_bounds__( 256, DECODE || NB == 16 ? 1 : NB == 8 ? 2 : 3 ) void attn_pages_f32_kernel( const T* __restrict__ q, T* __restrict__ out, Call a )
@@ -573,7 +573,9 @@ __global__ __launch_bounds__( 256, DECODE || NB == 16 ? 1 : NB == 8 ? 2 : 3 ) vo
 //   O^T += V^T P^T  16 x 16 x 32: the weights are the second operand as they lie, if slot 8 g + e is key 4 g + e (e < 4) and 16 + 4 g + e - 4; the first operand's
 //                   lanes take those keys of one dim with transposing LDS reads
 // 16-byte chunks of a row are swizzled by the row (in the address a lane fetches) so that both reads touch every bank once.
-// The weights are rounded to the storage type for the second product, as the matrix units take them; the sum takes them rounded too.
+// The weights are rounded to the storage type for the second product, as the matrix units take them; the sum takes them rounded too.  (In two parts, a second product or
+// the columns that up to 8 queries leave free, the error against 64 bits is the plain form's, 2.1e-4 for 2.7e-4 in f16, and 1.7e-3 for 2.4e-3 in bf16; 1 context of 301 keys
+// takes 7.2 us for 7.0, 16 of 500 9.7 for 9.4.)  An infinite value whose weight rounds to 0 makes NaN.
 // fp32: both products 16 x 16 x 4, a chunk of K being four of its steps, weights as they are, and V read value by value; 16 keys a stage above 64 elements.
 // (64 contexts of 100 to 4000 keys, 8 heads of 256 in fp32: 357 us, 6.0 TB/s; in the tile kernel above 1530.)
 // W waves of a work-group take the stages of one run in turns and are joined through LDS.
@@ -1261,9 +1263,10 @@ __global__ __launch_bounds__( 64 * W ) void attn_pages_decode_one_kernel( const 
 // for four pairs ahead and the second half of the exponentials computed beside the first pairs.
 // The weights are rounded to the storage type for the second product, as the matrix units take them; the sum takes them rounded too.
 // Blocks come longest first; where the kv heads are a multiple of 8 the blocks of a head go to one XCD, whose L2 then fetches its rows once.
-// A prompt of 4096 tokens, 8 kv heads of 128 with 8 queries each, f16: 284 to 289 us (0.96 PFLOP/s; matrix units busy half the time, the softmax a third, which do not
-// overlap fully with two waves a SIMD).  9 prompts of 1 to 1023 tokens behind 0 to 1500 keys, 32 heads, bf16: 97 us (0.62): a work-group begins with some 6 us of
-// dependent loads, and the last ones have a CU to themselves.
+// (What the rounding leaves would be a second product, half as many matrix instructions again where they bound the kernel.)
+// A prompt of 4096 tokens, 8 kv heads of 128 with 8 queries each, f16: 276 to 303 us on the cards seen (0.91 to 1.0 PFLOP/s; by counters the matrix units are busy half the
+// time, the vector ALU 0.3 of it, LDS reads a quarter, which do not overlap fully with two waves a SIMD).  9 prompts of 1 to 1023 tokens behind 0 to 1500 keys, 32 heads, bf16:
+// 97 us (0.62; matrix units 0.29): a work-group begins with some 6 us of dependent loads, and the last ones have a CU to themselves.
 // =================================================================================================
 typedef _Float16 f16x2 __attribute__( ( ext_vector_type( 2 ) ) );
 typedef __bf16 b16x2 __attribute__( ( ext_vector_type( 2 ) ) );

@@ -13,7 +13,7 @@
 // round, so that no two are equal and the lower index of equal values is the larger number, and are ranked by counting.  Where they are more than fit since many are equal
 // (a row that lets few tokens through is -inf elsewhere), the row is read again for what is larger and for as many of the equal ones as are wanted: 2047 rows of which
 // 30 of 32000 f16 values are finite, 20 alternatives, 102 us a call on its own (50 with all of them finite).  Where even what is larger is more than fit (a row whose
-// values are in order), the numbers come out one after the other, each the largest below the one before.
+// values are in order), the numbers come out one after the other, each the largest below the one before (2047 such rows, 20 alternatives: 1030 us).
 // Rows of one part are finished by their work-group.  Longer ones are cut into parts whose S, T, m and sorted largest numbers a second kernel joins.
 #include "gh_common.h"
 
@@ -461,8 +461,8 @@ void launch_logprobs( const LogprobPlan& p, const Outputs& o, const void* logits
   } else if ( pieces <= 2048 ) {
     go( many, std::integral_constant<int, 2> {} );
   } else if ( pieces <= 4096 ) {
-    // f16: more work-groups a CU, whose short phases fill each other's gaps (2047 rows of 32000, 20 alternatives: 40 us, with 1024 threads 46, with 256 43; 256 rows: 11.0 and
-    // 10.2; bf16 does not fit the registers so: 47 and 47)
+    // f16: more work-groups a CU, whose short phases fill each other's gaps (rows of 32000, 20 alternatives, calls with 512 and with 1024 threads, us: 384 rows 14.3 and 14.5, 448
+    // 14.6 and 15.2, 768 19.7 and 21.7, 2047 38.3 and 44.9, 4096 62.6 and 80.8; up to 320 equal.  256 threads, 2047 rows: 43.  bf16 does not fit the registers so: 47 and 47)
     if constexpr ( std::is_same_v<T, __half> ) {
       if ( rows >= 512 ) {
         go( std::integral_constant<int, 512> {}, std::integral_constant<int, 8> {} );
