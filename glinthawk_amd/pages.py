@@ -48,6 +48,9 @@ class PageBook:
             host_lib().glint_pages_delete(self._b)
             self._b = None
 
+    def __reduce__(self):
+        raise TypeError("a page book is not copied or pickled: two would delete the same pages")
+
     def _known(self, name: Hashable) -> int:
         if name not in self._ids:
             raise KeyError(name)

@@ -1,4 +1,6 @@
-"""Pages of a pool and the contexts that have them: several threads at once."""
+"""Pages of a pool and the contexts that have them: several threads at once, copies."""
+import copy
+import pickle
 import sys
 import threading
 
@@ -76,3 +78,12 @@ def test_one_name_that_threads_begin_at_once_is_one_context(fast_switches):
         book = PageBook(64, 4)
         together(lambda i: book.extend("a", 4), 4)
         assert book.length("a") == 16 and book.free() == 60, turn
+
+
+def test_copies_are_refused():
+    book = PageBook(9, 4)
+    book.extend("a", 5)
+    for make in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError, match="not copied"):
+            make(book)
+    assert book.line("a") == [0, 1] and book.free() == 7
